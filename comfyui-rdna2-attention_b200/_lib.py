@@ -55,7 +55,22 @@ SIGNATURES = {
     "b2_attn_decode_noalloc": (I, [P, P, P, P, P, I, I, I, I, F, P]),
     "b2_decode_step": (I, [P, I, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, F, ctypes.c_longlong, P]),
     "b2_decode_step_splits": (I, [I]),
+    "b2_rope": (I, [P, I64, I64, P, I64, I64, P, P, F, I, I, I, I, I, I, P]),
+    "b2_kv_append": (I, [P, I64, I64, P, I64, I64, P, P, I64, I64, I64, P, I, I, I, I, P, P, I, P, I64, I64, P, I64, I64,
+                         P, P, F, I, I, I, I, I, I, I, P]),
+    "b2_attn_ragged_workspace_bytes": (I64, [I, I, I, I]),
+    "b2_attn_ragged": (I, [P, P]),
 }
+
+
+class RaggedArgs(ctypes.Structure):
+    """b2_attn_ragged_args."""
+    _fields_ = ([("q", P), ("sqt", I64), ("sqh", I64), ("out", P), ("sot", I64), ("soh", I64), ("lse", P), ("k", P),
+                 ("v", P), ("s_page", I64), ("s_row", I64), ("s_head", I64), ("table", P), ("cu_q", P), ("lengths", P),
+                 ("prefix", P), ("slopes", P), ("workspace", P)]
+                + [(n, I) for n in ("table_ld", "max_pages", "num_pages", "page_size", "batch", "tokens", "key_rows",
+                                    "heads", "kv_heads", "dim", "dtype", "max_q", "causal", "window")]
+                + [("scale", F), ("softcap", F)])
 
 _lib = None
 
@@ -100,7 +115,8 @@ def require_cuda(*tensors):
 
 
 def device_status():
-    """Synchronizes and returns the device status bits that bounded waits set when they ran out (0 = none)."""
+    """Synchronizes and returns the device status bits that bounded waits set when they ran out and that a page
+    outside the cache sets (0 = none)."""
     flags = ctypes.c_uint(0)
     load().b2_device_status(ctypes.byref(flags))
     return flags.value

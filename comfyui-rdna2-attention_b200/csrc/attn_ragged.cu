@@ -1,0 +1,65 @@
+// C-ABI of the ragged attention: checks, then the kernel for the call's rows per kv head.
+#include "attn_ragged.cuh"
+
+using namespace b2;
+
+extern "C" int64_t b2_attn_ragged_workspace_bytes(int heads, int kv_heads, int dim, int max_q) {
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || (dim != 64 && dim != 128)) return 0;
+    (void)max_q;
+    return rows_workspace(dim);
+}
+
+extern "C" int b2_attn_ragged(const b2_attn_ragged_args* p, void* stream) {
+    if (!p) return fail(B2_ERR_INVALID, "attn_ragged: null arguments");
+    if (p->batch < 0 || p->tokens < 0 || p->heads <= 0 || p->kv_heads <= 0 || p->heads % p->kv_heads || p->window < 0 ||
+        p->key_rows < 0 || p->max_pages < 0 || p->num_pages < 0 || p->table_ld < 0)
+        return fail(B2_ERR_INVALID, "attn_ragged: bad shape batch=%d tokens=%d heads=%d kv_heads=%d window=%d", p->batch,
+                    p->tokens, p->heads, p->kv_heads, p->window);
+    if (p->dim != 64 && p->dim != 128) return fail(B2_ERR_UNSUPPORTED, "attn_ragged: head dim %d (64 or 128)", p->dim);
+    if (p->dtype != B2_F16 && p->dtype != B2_BF16)
+        return fail(B2_ERR_UNSUPPORTED, "attn_ragged: dtype code %d (fp16 or bf16)", p->dtype);
+    if (!(p->scale > 0.f) || p->scale > 3e38f || !(p->softcap >= 0.f) || p->softcap > 3e38f)
+        return fail(B2_ERR_INVALID, "attn_ragged: scale must be positive and softcap not negative, both finite");
+    if ((int64_t)p->tokens * p->heads > (1 << 30))
+        return fail(B2_ERR_UNSUPPORTED, "attn_ragged: %d tokens of %d heads in one call", p->tokens, p->heads);
+    if (p->batch == 0 || p->tokens == 0) return B2_OK;
+    if (!p->q || !p->out || !p->k || !p->v || !p->cu_q || !p->lengths || !p->workspace)
+        return fail(B2_ERR_INVALID, "attn_ragged: null pointer");
+    if (p->table && p->page_size <= 0) return fail(B2_ERR_INVALID, "attn_ragged: page size %d", p->page_size);
+    if (!aligned16(p->q) || !aligned16(p->out) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->workspace) ||
+        (p->sqt | p->sqh | p->sot | p->soh | p->s_page | p->s_row | p->s_head) % 8)
+        return fail(B2_ERR_UNSUPPORTED, "attn_ragged: q, k, v and out must be 16-byte aligned with 16-byte strides");
+    RaggedArgs a{};
+    a.q = p->q;
+    a.sqt = p->sqt;
+    a.sqh = p->sqh;
+    a.out = p->out;
+    a.sot = p->sot;
+    a.soh = p->soh;
+    a.lse = p->lse;
+    a.k = p->k;
+    a.v = p->v;
+    a.s_page = p->s_page;
+    a.s_row = p->s_row;
+    a.s_head = p->s_head;
+    a.table = p->table;
+    a.table_ld = p->table_ld;
+    a.max_pages = p->max_pages;
+    a.num_pages = p->num_pages;
+    a.page_size = p->page_size;
+    a.cu_q = p->cu_q;
+    a.lengths = p->lengths;
+    a.prefix = p->prefix;
+    a.slopes = p->slopes;
+    a.batch = p->batch;
+    a.tokens = p->tokens;
+    a.key_rows = p->key_rows;
+    a.heads = p->heads;
+    a.kv_heads = p->kv_heads;
+    a.group = p->heads / p->kv_heads;
+    a.causal = p->causal != 0;
+    a.window = p->window >= (1 << 30) ? 0 : p->window;  // no position reaches that far
+    a.scale = p->scale;
+    a.softcap = p->softcap;
+    return attn_rows(a, p->dim, p->dtype == B2_BF16, p->workspace, (cudaStream_t)stream);
+}

@@ -1,0 +1,368 @@
+// What the two ragged attention kernels (attn_rows.cu, attn_tiles.cu) share: the problem, the visible keys of a row,
+// and how the work is dealt to the CTAs.
+//
+// Sequence b has n new tokens (rows cu_q[b] .. cu_q[b + 1] of q) and len keys, the last n of them the tokens' own:
+// token i sits at position pos = len - n + i. It sees the keys [lo, hi):
+//   hi = len, or with the causal mask min(len, max(pos + 1, prefix[b]));   lo = max(0, pos - window + 1), or 0.
+// The G = H / Hkv query heads of a kv head share its keys, so they are packed into rows: row r of (b, kv head) is token
+// r / G, head r % G, and an item is ROWS consecutive rows. An item's keys are cut into units of UNIT keys (at least one
+// unit, so that an item that sees nothing still writes its zeros).
+//
+// The lengths live on the device (a captured graph replays with other lengths), so the CTAs deal the work among
+// themselves: all units, ordered by (sequence, kv head, row tile, key), are cut into gridDim.x runs of equal length,
+// each CTA adds up the sequences' units and finds its run. A run holds whole items, and at its ends parts of items,
+// which leave unnormalized results (O, and per row the maximum m and the sum l) in the CTA's two slots of the workspace:
+// slot 2x for the part of an item that began in an earlier CTA, slot 2x + 1 for the head of an item that goes on in
+// the next. merge_kernel joins each head with the parts that follow it, in CTA order, so results do not depend on timing.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "host.hpp"
+
+namespace b2 {
+
+constexpr float RAGGED_LOG2E = 1.4426950408889634f;
+
+struct RaggedArgs {
+    const void* q;
+    int64_t sqt, sqh;
+    void* out;
+    int64_t sot, soh;
+    float* lse;  // [tokens, heads], may be null
+    const void *k, *v;
+    int64_t s_page, s_row, s_head;  // packed keys: s_page unused
+    const int32_t* table;           // null: packed keys
+    int table_ld, max_pages, num_pages, page_size;
+    const int32_t* cu_q;
+    const int32_t* lengths;  // paged: keys per sequence; packed: cu_k
+    const int32_t* prefix;   // null: none
+    const float* slopes;     // null: none
+    int batch, tokens, key_rows, heads, kv_heads, group;
+    int causal, window;
+    float scale, softcap;
+    // workspace: partial O [slots][ROWS][D], (m, l) [slots][ROWS], item descriptor [CTAs][4]
+    float* part_o;
+    float2* part_ml;
+    int4* desc;
+};
+
+struct Sequence {
+    int q0, n, len, pos0, prefix;
+    int64_t key0;  // packed keys: first row
+};
+
+__device__ __forceinline__ Sequence load_sequence(const RaggedArgs& a, int b) {
+    Sequence s;
+    s.q0 = min(max(a.cu_q[b], 0), a.tokens);
+    s.n = max(min(a.cu_q[b + 1], a.tokens) - s.q0, 0);
+    s.key0 = 0;
+    if (a.table) {
+        s.len = max(a.lengths[b], 0);
+        s.len = (int)min((int64_t)s.len, (int64_t)a.max_pages * a.page_size);  // no key lies behind the table
+    } else {
+        const int k0 = min(max(a.lengths[b], 0), a.key_rows);
+        s.len = max(min(a.lengths[b + 1], a.key_rows) - k0, 0);
+        s.key0 = k0;
+    }
+    s.pos0 = s.len - s.n;
+    s.prefix = a.prefix ? min(max(a.prefix[b], 0), s.len) : 0;
+    return s;
+}
+
+__device__ __forceinline__ int key_hi(const RaggedArgs& a, const Sequence& s, int tok) {
+    return a.causal ? min(s.len, max(s.pos0 + tok + 1, s.prefix)) : s.len;
+}
+__device__ __forceinline__ int key_lo(const RaggedArgs& a, const Sequence& s, int tok) {
+    return a.window ? max(0, s.pos0 + tok - a.window + 1) : 0;
+}
+
+// The units [u0, u1) of the keys that any row of row tile rt sees.
+template <int ROWS, int UNIT>
+__device__ __forceinline__ int2 item_units(const RaggedArgs& a, const Sequence& s, int rt) {
+    const int tok0 = rt * ROWS / a.group;
+    const int tok1 = min(s.n - 1, (rt * ROWS + ROWS - 1) / a.group);
+    const int hi = key_hi(a, s, tok1), lo = key_lo(a, s, tok0);
+    if (hi <= lo) return make_int2(0, 1);
+    return make_int2(lo / UNIT, (hi + UNIT - 1) / UNIT);
+}
+template <int ROWS>
+__device__ __forceinline__ int row_tiles(const RaggedArgs& a, const Sequence& s) {
+    return (s.n * a.group + ROWS - 1) / ROWS;
+}
+// Units of one kv head of a sequence.
+template <int ROWS, int UNIT>
+__device__ __forceinline__ int64_t head_units(const RaggedArgs& a, const Sequence& s) {
+    int64_t c = 0;
+    const int tiles = row_tiles<ROWS>(a, s);
+    for (int rt = 0; rt < tiles; ++rt) {
+        const int2 u = item_units<ROWS, UNIT>(a, s, rt);
+        c += u.y - u.x;
+    }
+    return c;
+}
+
+// The runs: run x is [begin(x), begin(x + 1)) of all units.
+struct Runs {
+    int64_t total;
+    int count;
+    __device__ __forceinline__ int64_t begin(int x) const { return total / count * x + total % count * x / count; }
+};
+
+// A CTA's place in the work: item (b, kvh, rt) with units [u0, u1), the next one to do and how many are left in its run.
+struct Cursor {
+    Sequence s;
+    int b, kvh, rt, u0, u1, unit;
+    int64_t left;
+    Runs runs;
+};
+
+// Finds the CTA's run with all of its threads (THREADS of them; smem: 40 int64). Every thread returns the same cursor.
+template <int ROWS, int UNIT, int THREADS>
+__device__ __forceinline__ Cursor find_run(const RaggedArgs& a, int64_t* smem) {
+    constexpr int WARPS = THREADS / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto units_of = [&](int b) -> int64_t {
+        return b < a.batch ? head_units<ROWS, UNIT>(a, load_sequence(a, b)) * a.kv_heads : 0;
+    };
+    // Total, and each thread's count for the first THREADS sequences.
+    const int64_t first = units_of(tid);
+    int64_t sum = first;
+    for (int b = tid + THREADS; b < a.batch; b += THREADS) sum += units_of(b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) smem[warp] = sum;
+    if (tid == 0) smem[34] = -1;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) total += smem[w];
+    // Fewer units than CTAs: one each, the other CTAs have none.
+    Cursor c;
+    c.runs.total = total;
+    c.runs.count = (int)min((int64_t)gridDim.x, total);
+    c.left = 0;
+    c.b = c.kvh = c.rt = c.u0 = c.u1 = c.unit = 0;
+    c.s = Sequence{};
+    __syncthreads();
+    if ((int)blockIdx.x >= c.runs.count) return c;
+    const int64_t begin = c.runs.begin(blockIdx.x);
+    c.left = c.runs.begin(blockIdx.x + 1) - begin;
+    // The sequence that holds unit `begin`: prefix sums over THREADS sequences at a time.
+    int64_t before = 0;
+    for (int base = 0;; base += THREADS) {
+        const int64_t mine = base == 0 ? first : units_of(base + tid);
+        int64_t inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += up;
+        }
+        if (lane == 31) smem[warp] = inc;
+        __syncthreads();
+        int64_t off = before;
+        for (int w = 0; w < warp; ++w) off += smem[w];
+        const int64_t lo = off + inc - mine;
+        if (mine > 0 && lo <= begin && begin < lo + mine) {
+            smem[34] = base + tid;
+            smem[35] = begin - lo;
+        }
+        for (int w = 0; w < WARPS; ++w) before += smem[w];
+        __syncthreads();
+        if (smem[34] >= 0 || base + THREADS >= a.batch) break;
+    }
+    c.b = (int)smem[34];
+    int64_t rem = smem[35];
+    if (c.b < 0) {  // not reached: begin < total
+        c.left = 0;
+        c.b = 0;
+        return c;
+    }
+    c.s = load_sequence(a, c.b);
+    const int64_t per_head = head_units<ROWS, UNIT>(a, c.s);
+    c.kvh = (int)(rem / per_head);
+    rem -= c.kvh * per_head;
+    for (c.rt = 0;; ++c.rt) {
+        const int2 u = item_units<ROWS, UNIT>(a, c.s, c.rt);
+        if (rem < u.y - u.x) {
+            c.u0 = u.x;
+            c.u1 = u.y;
+            c.unit = u.x + (int)rem;
+            break;
+        }
+        rem -= u.y - u.x;
+    }
+    return c;
+}
+
+// Moves on by `done` units, to the next item where the current one is finished.
+template <int ROWS, int UNIT>
+__device__ __forceinline__ void advance(const RaggedArgs& a, Cursor& c, int done) {
+    c.unit += done;
+    c.left -= done;
+    if (c.unit < c.u1 || c.left <= 0) return;
+    if (++c.rt >= row_tiles<ROWS>(a, c.s)) {
+        c.rt = 0;
+        if (++c.kvh >= a.kv_heads) {
+            c.kvh = 0;
+            do {
+                if (c.b + 1 >= a.batch) {  // not reached: units are left
+                    c.left = 0;
+                    return;
+                }
+                c.s = load_sequence(a, ++c.b);
+            } while (c.s.n == 0);
+        }
+    }
+    const int2 u = item_units<ROWS, UNIT>(a, c.s, c.rt);
+    c.u0 = c.unit = u.x;
+    c.u1 = u.y;
+}
+
+// The descriptor the merge reads: how many of the next CTAs hold the rest of an item that this CTA's run ends inside
+// (`end`: where this run stops in the item), 0 where it does not.
+__device__ __forceinline__ int parts_after(const Cursor& c, int end) {
+    if (end >= c.u1) return 0;
+    const int64_t stop = c.runs.begin(blockIdx.x + 1) + (c.u1 - end);
+    int n = 1;
+    while (blockIdx.x + 1 + n < c.runs.count && c.runs.begin(blockIdx.x + 1 + n) < stop) ++n;
+    return n;
+}
+
+// Element offset of a key row of the sequence in k and v (head 0), or -1: behind the last key, or on a page that does
+// not exist (reported in *status; the row then counts as zeros).
+__device__ __forceinline__ int64_t key_row_offset(const RaggedArgs& a, const Sequence& s, int b, int key,
+                                                  unsigned int* status) {
+    if (key >= s.len) return -1;
+    if (!a.table) return (s.key0 + key) * a.s_row;
+    const int pi = key / a.page_size;
+    const int page = a.table[(int64_t)b * a.table_ld + pi];
+    if (page < 0 || page >= a.num_pages) {
+        atomicOr(status, B2_DEV_BAD_PAGE);
+        return -1;
+    }
+    return (int64_t)page * a.s_page + (int64_t)(key - pi * a.page_size) * a.s_row;
+}
+
+// cap * tanh(x / cap) in the base-2 domain: tanh(y) = 1 - 2 / (1 + 2^(2 y log2 e)). y2 = 2 x log2(e) / cap,
+// cap2 = cap log2(e); saturates to +-cap2 when the power over- or underflows.
+__device__ __forceinline__ float capped(float y2, float cap2) {
+    return fmaf(-2.f * cap2, rcp_approx(1.f + ex2_approx(y2)), cap2);
+}
+
+template <class T>
+struct Pair;  // two 16-bit values of T from fp32, rounded to nearest even
+template <>
+struct Pair<__half> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { return h2_as_u32(__floats2half2_rn(a, b)); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+
+// Natural logarithm of a row's sum of exponentials from its base-2 maximum and sum; -inf where nothing was seen.
+__device__ __forceinline__ float log_sum(float m2, float l) {
+    return l == 0.f ? -INFINITY : (m2 + log2f(l)) * 0.69314718055994531f;
+}
+
+// Joins the parts of every item that was cut: one warp per row, blockIdx.x = the CTA that holds the item's head.
+//   M = max m_p, L = sum l_p 2^(m_p - M), out = sum O_p 2^(m_p - M) / L
+template <class T, int D, int ROWS>
+__global__ void __launch_bounds__(512) merge_kernel(const RaggedArgs a) {
+    pdl_wait();
+    const int x = blockIdx.x, lane = threadIdx.x & 31;
+    const int row = blockIdx.y * 16 + (threadIdx.x >> 5);
+    const int4 d = a.desc[x];  // parts after the head, b, kvh, rt
+    if (d.x == 0) return;
+    const Sequence s = load_sequence(a, d.y);
+    const int r = d.w * ROWS + row;
+    if (r >= s.n * a.group) return;
+    const int parts = d.x + 1;
+    auto slot = [&](int p) { return (int64_t)(p == 0 ? 2 * x + 1 : 2 * (x + p)) * ROWS + row; };
+    float M = -INFINITY;
+    for (int p = lane; p < parts; p += 32) M = fmaxf(M, a.part_ml[slot(p)].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float ref = M == -INFINITY ? 0.f : M;
+    constexpr int C = D / 32;
+    float acc[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) acc[i] = 0.f;
+    float L = 0.f;
+    for (int p0 = 0; p0 < parts; p0 += 32) {
+        float w = 0.f;
+        if (p0 + lane < parts) {
+            const float2 ml = a.part_ml[slot(p0 + lane)];
+            w = ex2_approx(ml.x - ref);
+            L += w * ml.y;
+        }
+        const int here = min(32, parts - p0);
+#pragma unroll 4
+        for (int p = 0; p < here; ++p) {
+            const float wp = __shfl_sync(0xffffffffu, w, p);
+            const float* src = a.part_o + slot(p0 + p) * D + lane * C;
+            float v[C];
+            if constexpr (C == 4)
+                *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+            else
+                *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+            for (int i = 0; i < C; ++i) acc[i] = fmaf(wp, v[i], acc[i]);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int tok = s.q0 + r / a.group, head = d.z * a.group + r % a.group;
+    T* dst = static_cast<T*>(a.out) + (int64_t)tok * a.sot + (int64_t)head * a.soh + lane * C;
+    uint32_t u[C / 2];
+#pragma unroll
+    for (int i = 0; i < C / 2; ++i) u[i] = Pair<T>::pack(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    if constexpr (C == 4)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(u[0], u[1]);
+    else
+        *reinterpret_cast<uint32_t*>(dst) = u[0];
+    if (a.lse && lane == 0) a.lse[(int64_t)tok * a.heads + head] = log_sum(M, L);
+}
+  // two 16-bit values of T from fp32, rounded to nearest even
+
+// ---------------------------------------------------------------- host
+// Workspace of a launch of `ctas` CTAs: two slots each of ROWS rows of O and (m, l), and the descriptors.
+inline int64_t ragged_workspace(int ctas, int rows, int dim) {
+    return (int64_t)ctas * (2 * rows * (dim * 4 + 8) + 16);
+}
+inline void ragged_slots(RaggedArgs& a, void* workspace, int ctas, int rows, int dim) {
+    unsigned char* w = static_cast<unsigned char*>(workspace);
+    a.part_o = reinterpret_cast<float*>(w);
+    w += (int64_t)ctas * 2 * rows * dim * 4;
+    a.part_ml = reinterpret_cast<float2*>(w);
+    w += (int64_t)ctas * 2 * rows * 8;
+    a.desc = reinterpret_cast<int4*>(w);
+}
+// The merge starts while the attention's last CTAs finish (programmatic stream serialization); it reads nothing of
+// theirs before griddepcontrol.wait.
+template <class K>
+int launch_merge(K kernel, const RaggedArgs& a, int ctas, int rows, cudaStream_t s) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas, rows / 16);
+    cfg.blockDim = dim3(512);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    if (e != cudaSuccess) return fail(B2_ERR_CUDA, "merge_kernel: %s", cudaGetErrorString(e));
+    return B2_OK;
+}
+
+// The two kernels' launchers (attn_rows.cu, attn_tiles.cu).
+int64_t rows_workspace(int dim);
+int attn_rows(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t s);
+
+}  // namespace b2

@@ -86,9 +86,11 @@ const char* b2_last_error(void) { return b2::g_message; }
 int b2_device_status(unsigned int* flags) {
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return b2::fail(B2_ERR_CUDA, "cudaDeviceSynchronize: %s", cudaGetErrorString(e));
-    unsigned int f = b2::read_status_gemm() | b2::read_status_attention() | b2::read_status_gemm_w4a8();
+    unsigned int f = b2::read_status_gemm() | b2::read_status_attention() | b2::read_status_gemm_w4a8() |
+                     b2::read_status_rope() | b2::read_status_attn_rows();
     if (flags) *flags = f;
-    if (f) return b2::fail(B2_ERR_DEVICE, "device status 0x%x: a bounded wait ran out", f);
+    if (f) return b2::fail(B2_ERR_DEVICE, "device status 0x%x: %s", f,
+                              f == B2_DEV_BAD_PAGE ? "a page table entry outside the cache" : "a bounded wait ran out");
     return B2_OK;
 }
 

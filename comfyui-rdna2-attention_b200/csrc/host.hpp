@@ -53,5 +53,7 @@ inline int set_smem(K kernel, int bytes) {
 unsigned int read_status_gemm();
 unsigned int read_status_attention();
 unsigned int read_status_gemm_w4a8();
+unsigned int read_status_rope();
+unsigned int read_status_attn_rows();
 
 }  // namespace b2

@@ -1,0 +1,325 @@
+// Rotary positions of packed rows, alone (b2_rope) or on the way of new keys and values into a paged cache
+// (b2_kv_append).
+//
+// A head's first 2F values are F pairs; pair f of a token at position p turns by the angle p * inv_freq[f]:
+//   a' = mscale (a cos - b sin),   b' = mscale (a sin + b cos)
+// with (a, b) = (x[f], x[F + f]) in the half layout and (x[2f], x[2f + 1]) in the interleaved one; the values from 2F
+// on pass through. The angle is formed and reduced to a quarter turn in 64 bits (a position of 10^6 times a frequency
+// has only four bits of the turn's fraction left in 32), sine and cosine of the remainder in 32, and each result is
+// rounded once, to the tensor's type.
+//
+// Bound by HBM: each value is read once and written once. One CTA per token: its F sines and cosines are computed once,
+// into shared memory, and every head's pairs use them. A thread's item is 16 bytes of a's and 16 bytes of b's (both
+// layouts: the same F indices), loaded before the angles are known so that the two latencies overlap.
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "host.hpp"
+
+namespace b2 {
+namespace {
+
+__device__ unsigned int g_status;
+
+constexpr int MAX_PAIRS = 512;
+
+struct RopeArgs {
+    // rows rotated from x to out: rope's tensor, or the queries beside appended keys
+    const void* x;
+    void* out;
+    int64_t sxt, sxh, sot, soh;  // element strides of token and head
+    int heads;
+    // appended keys and values (kv_heads 0: none)
+    const void *k, *v;
+    void *k_cache, *v_cache;
+    int64_t skt, skh, svt, svh, sc_page, sc_row, sc_head;
+    int kv_heads;
+    const int32_t *table, *cu_q, *lengths;
+    int batch, table_ld, max_pages, num_pages, page_size;
+    const int64_t* positions;  // null: the cache position
+    const float* inv_freq;
+    float mscale;
+    int tokens, dim, pairs;
+};
+
+template <class T>
+__device__ __forceinline__ float to_f(T v) {
+    return static_cast<float>(v);
+}
+template <class T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) {
+    return v;
+}
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) {
+    return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+// V values as one load: 16 bytes (V * sizeof(T) == 16) or a single value.
+template <class T, int V>
+struct alignas(V == 1 ? sizeof(T) : 16) Vec {
+    T e[V];
+};
+
+// The sequence of row r: the b with cu_q[b] <= r < cu_q[b + 1], or -1 (rows behind the last sequence). A warp looks at
+// 32 borders at a time. All lanes return the same value.
+__device__ __forceinline__ int find_sequence(const int32_t* cu_q, int batch, int r) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = batch;  // cu_q[lo] <= r is known (or lo = 0), cu_q[hi] > r is to be found
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int at = min(lo + (lane + 1) * step, hi);
+        const unsigned past = __ballot_sync(0xffffffffu, cu_q[at] > r);
+        if (!past) return -1;
+        const int first = __ffs(past) - 1;
+        hi = min(lo + (first + 1) * step, hi);
+        lo = lo + first * step;
+    }
+    return (cu_q[lo] <= r && r < cu_q[lo + 1]) ? lo : -1;
+}
+
+template <class T, int V, bool INTER>
+__global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
+    __shared__ float s_cos[MAX_PAIRS], s_sin[MAX_PAIRS];
+    const int t = blockIdx.x;
+    using W = Vec<T, V>;
+    const int per_head = a.dim / (2 * V);
+    const int rot_items = a.pairs / V;
+    const int items = (a.heads + 2 * a.kv_heads) * per_head;
+
+    int64_t pos = 0;
+    int64_t slot = -1;
+    if (a.kv_heads) {
+        const int b = find_sequence(a.cu_q, a.batch, t);
+        if (b < 0) return;
+        const int64_t p = (int64_t)a.lengths[b] - a.cu_q[b + 1] + t;
+        pos = p;
+        if (p >= 0) {  // below 2^31: t < cu_q[b + 1]
+            const int pi = (int)p / a.page_size;
+            const int page = pi < a.max_pages ? a.table[(int64_t)b * a.table_ld + pi] : -1;
+            if (page >= 0 && page < a.num_pages) slot = (int64_t)page * a.sc_page + ((int)p - pi * a.page_size) * a.sc_row;
+        }
+        if (slot < 0 && threadIdx.x == 0) atomicOr(&g_status, B2_DEV_BAD_PAGE);
+    }
+    if (a.positions) pos = a.positions[t];
+
+    struct Item {
+        const T* src;
+        T* dst;
+        int off_a, off_b, f;
+        bool rotate, live;
+    };
+    auto item = [&](int i) {
+        Item m;
+        m.live = i < items;
+        if (!m.live) return m;
+        const int head = i / per_head, u = i - head * per_head;
+        m.rotate = u < rot_items && head < a.heads + a.kv_heads;
+        m.f = u * V;
+        if (u < rot_items && !INTER) {
+            m.off_a = u * V;
+            m.off_b = a.pairs + u * V;
+        } else {
+            m.off_a = 2 * u * V;
+            m.off_b = m.off_a + V;
+        }
+        if (head < a.heads) {
+            m.src = static_cast<const T*>(a.x) + (int64_t)t * a.sxt + head * a.sxh;
+            m.dst = static_cast<T*>(a.out) + (int64_t)t * a.sot + head * a.soh;
+        } else {
+            const bool is_k = head < a.heads + a.kv_heads;
+            const int h = head - a.heads - (is_k ? 0 : a.kv_heads);
+            m.src = is_k ? static_cast<const T*>(a.k) + (int64_t)t * a.skt + h * a.skh
+                         : static_cast<const T*>(a.v) + (int64_t)t * a.svt + h * a.svh;
+            m.dst = static_cast<T*>(is_k ? a.k_cache : a.v_cache) + slot + h * a.sc_head;
+            m.live = slot >= 0;
+        }
+        return m;
+    };
+    auto load = [](const Item& m, W& wa, W& wb) {
+        if (m.live) {
+            wa = *reinterpret_cast<const W*>(m.src + m.off_a);
+            wb = *reinterpret_cast<const W*>(m.src + m.off_b);
+        }
+    };
+    auto finish = [&](const Item& m, W& wa, W& wb) {
+        if (!m.live) return;
+        if (m.rotate) {
+            float x[2 * V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                x[e] = to_f(wa.e[e]);
+                x[V + e] = to_f(wb.e[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float c = s_cos[m.f + e], s = s_sin[m.f + e];
+                const int ia = INTER ? 2 * e : e, ib = INTER ? 2 * e + 1 : V + e;
+                const float p = x[ia], q = x[ib];
+                x[ia] = p * c - q * s;
+                x[ib] = p * s + q * c;
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                wa.e[e] = from_f<T>(x[e]);
+                wb.e[e] = from_f<T>(x[V + e]);
+            }
+        }
+        *reinterpret_cast<W*>(m.dst + m.off_a) = wa;
+        *reinterpret_cast<W*>(m.dst + m.off_b) = wb;
+    };
+
+    W wa, wb;
+    Item m = item(threadIdx.x);
+    load(m, wa, wb);
+    for (int f = threadIdx.x; f < a.pairs; f += blockDim.x) {
+        // turns = p * inv_freq / (2 pi), less its nearest quarter turn: |rest| <= 1/8
+        const double turns = (double)pos * (double)a.inv_freq[f] * 0.15915494309189533577;
+        const double frac = turns - rint(turns);
+        const double quarter = rint(4.0 * frac);
+        const int qn = (int)quarter & 3;
+        float s, c;
+        sincospif((float)(2.0 * (frac - 0.25 * quarter)), &s, &c);
+        const float cc = (qn & 1) ? -s : c, ss = (qn & 1) ? c : s;  // one quarter turn: (cos, sin) -> (-sin, cos)
+        s_cos[f] = ((qn & 2) ? -cc : cc) * a.mscale;
+        s_sin[f] = ((qn & 2) ? -ss : ss) * a.mscale;
+    }
+    __syncthreads();
+    finish(m, wa, wb);
+    for (int i = threadIdx.x + blockDim.x; i < items; i += blockDim.x) {
+        m = item(i);
+        load(m, wa, wb);
+        finish(m, wa, wb);
+    }
+}
+
+template <class T>
+int launch(const RopeArgs& a, bool wide, bool inter, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const int items = (a.heads + 2 * a.kv_heads) * (a.dim / (wide ? 2 * V : 2));
+    const int threads = items <= 64 && a.pairs <= 64 ? 64 : items <= 128 ? 128 : 256;
+    if (wide) {
+        if (inter)
+            rope_kernel<T, V, true><<<a.tokens, threads, 0, s>>>(a);
+        else
+            rope_kernel<T, V, false><<<a.tokens, threads, 0, s>>>(a);
+    } else {
+        if (inter)
+            rope_kernel<T, 1, true><<<a.tokens, threads, 0, s>>>(a);
+        else
+            rope_kernel<T, 1, false><<<a.tokens, threads, 0, s>>>(a);
+    }
+    return check_launch("rope_kernel");
+}
+
+int run(const RopeArgs& a, int dtype, int inter, void* stream, const char* what) {
+    if (a.dim <= 0 || a.dim % 2 || a.pairs < 0 || 2 * a.pairs > a.dim || a.pairs > MAX_PAIRS)
+        return fail(B2_ERR_UNSUPPORTED, "%s: head dim %d with %d rotated pairs (dim even, 2 * pairs <= dim, pairs <= %d)", what,
+                    a.dim, a.pairs, MAX_PAIRS);
+    if (a.pairs && !a.inv_freq) return fail(B2_ERR_INVALID, "%s: null inv_freq", what);
+    if (dtype < B2_F16 || dtype > B2_F32) return fail(B2_ERR_UNSUPPORTED, "%s: dtype code %d", what, dtype);
+    const int size = dtype == B2_F32 ? 4 : 2;
+    const int vec = 16 / size;
+    // 16-byte items need every row and both halves of a pair on 16 bytes; any other shape goes value by value.
+    bool wide = a.pairs % vec == 0 && a.dim % (2 * vec) == 0;
+    if (a.heads) wide = wide && aligned16(a.x) && aligned16(a.out) && (a.sxt | a.sxh | a.sot | a.soh) % vec == 0;
+    if (a.kv_heads)
+        wide = wide && aligned16(a.k) && aligned16(a.v) && aligned16(a.k_cache) && aligned16(a.v_cache) &&
+               (a.skt | a.skh | a.svt | a.svh | a.sc_page | a.sc_row | a.sc_head) % vec == 0;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == B2_F16) return launch<__half>(a, wide, inter != 0, s);
+    if (dtype == B2_BF16) return launch<__nv_bfloat16>(a, wide, inter != 0, s);
+    return launch<float>(a, wide, inter != 0, s);
+}
+
+}  // namespace
+
+unsigned int read_status_rope() {
+    unsigned int v = 0, zero = 0;
+    cudaMemcpyFromSymbol(&v, g_status, sizeof(v));
+    if (v) cudaMemcpyToSymbol(g_status, &zero, sizeof(zero));
+    return v;
+}
+
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" int b2_rope(const void* x, int64_t sxt, int64_t sxh, void* out, int64_t sot, int64_t soh,
+                       const int64_t* positions, const float* inv_freq, float mscale, int tokens, int heads, int dim,
+                       int pairs, int interleaved, int dtype, void* stream) {
+    if (tokens < 0 || heads < 0) return fail(B2_ERR_INVALID, "rope: bad shape tokens=%d heads=%d", tokens, heads);
+    if (tokens == 0 || heads == 0) return B2_OK;
+    if (!x || !out || !positions) return fail(B2_ERR_INVALID, "rope: null pointer");
+    RopeArgs a{};
+    a.x = x;
+    a.out = out;
+    a.sxt = sxt;
+    a.sxh = sxh;
+    a.sot = sot;
+    a.soh = soh;
+    a.heads = heads;
+    a.positions = positions;
+    a.inv_freq = inv_freq;
+    a.mscale = mscale;
+    a.tokens = tokens;
+    a.dim = dim;
+    a.pairs = pairs;
+    return run(a, dtype, interleaved, stream, "rope");
+}
+
+extern "C" int b2_kv_append(const void* k, int64_t skt, int64_t skh, const void* v, int64_t svt, int64_t svh, void* k_cache,
+                            void* v_cache, int64_t s_page, int64_t s_row, int64_t s_head, const int32_t* table, int table_ld,
+                            int max_pages, int num_pages, int page_size, const int32_t* cu_q, const int32_t* lengths,
+                            int batch, const void* q, int64_t sqt, int64_t sqh, void* q_out, int64_t sot, int64_t soh,
+                            const int64_t* positions, const float* inv_freq, float mscale, int tokens, int heads,
+                            int kv_heads, int dim, int pairs, int interleaved, int dtype, void* stream) {
+    if (tokens < 0 || heads < 0 || kv_heads <= 0 || batch < 0 || max_pages < 0 || num_pages < 0 || page_size <= 0 ||
+        table_ld < 0)
+        return fail(B2_ERR_INVALID, "kv_append: bad shape tokens=%d heads=%d kv_heads=%d batch=%d pages %d of %d, page size %d",
+                    tokens, heads, kv_heads, batch, max_pages, num_pages, page_size);
+    if (tokens == 0 || batch == 0) return B2_OK;
+    if (!k || !v || !k_cache || !v_cache || !table || !cu_q || !lengths || (heads && (!q || !q_out)))
+        return fail(B2_ERR_INVALID, "kv_append: null pointer");
+    RopeArgs a{};
+    a.x = q;
+    a.out = q_out;
+    a.sxt = sqt;
+    a.sxh = sqh;
+    a.sot = sot;
+    a.soh = soh;
+    a.heads = heads;
+    a.k = k;
+    a.v = v;
+    a.k_cache = k_cache;
+    a.v_cache = v_cache;
+    a.skt = skt;
+    a.skh = skh;
+    a.svt = svt;
+    a.svh = svh;
+    a.sc_page = s_page;
+    a.sc_row = s_row;
+    a.sc_head = s_head;
+    a.kv_heads = kv_heads;
+    a.table = table;
+    a.table_ld = table_ld;
+    a.max_pages = max_pages;
+    a.num_pages = num_pages;
+    a.page_size = page_size;
+    a.cu_q = cu_q;
+    a.lengths = lengths;
+    a.batch = batch;
+    a.positions = positions;
+    a.inv_freq = inv_freq;
+    a.mscale = mscale;
+    a.tokens = tokens;
+    a.dim = dim;
+    a.pairs = pairs;
+    return run(a, dtype, interleaved, stream, "kv_append");
+}

@@ -584,5 +584,262 @@ def decode_step(table, x, x2, qkv, att, act, partial, stats, inv_freq, pos, leng
     return x
 
 
+# ---------------------------------------------------------------- rotary positions, paged cache, packed sequences
+_DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+MAX_ROPE_PAIRS = 512
+BAD_PAGE = 16  # bit of _lib.device_status(): a page outside the cache was skipped
+
+
+def _on(t, fn):
+    """fn() with t's device current (the launch then goes to torch's current stream of that device)."""
+    if t.device.index == torch.cuda.current_device():
+        return fn()
+    with torch.cuda.device(t.device):
+        return fn()
+
+
+def _one_device(t, *others):
+    require_cuda(t, *others)
+    for o in others:
+        if o is not None and o.device != t.device:
+            _fail(f"tensors on {t.device} and {o.device}: one call takes one device")
+
+
+def _packed(t, name, like=None, dtypes=(torch.float16, torch.bfloat16, torch.float32)):
+    """[tokens, heads, dim] with a contiguous last dimension; ``like`` gives the dtype."""
+    if t.dim() != 3 or t.stride(2) != 1:
+        _fail(f"{name} must be [tokens, heads, dim] with a contiguous last dimension")
+    if t.dtype not in dtypes or (like is not None and t.dtype != like.dtype):
+        _fail(f"{name} has dtype {t.dtype}, needs {like.dtype if like is not None else ' or '.join(map(str, dtypes))}")
+
+
+def _ints(t, n, name):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        _fail(f"{name} must be contiguous int32 [{n}] (got {t.dtype}, {tuple(t.shape)})")
+
+
+def _cache(k_cache, v_cache, table, kv_heads, dim, like, name):
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if t.dim() != 4 or t.shape[2] != kv_heads or t.shape[3] != dim or t.stride(3) != 1 or t.dtype != like.dtype:
+            _fail(f"{name}: {n} must be {like.dtype} [pages, page_size, {kv_heads}, {dim}] with a contiguous last dimension")
+    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+        _fail(f"{name}: k_cache and v_cache must have equal shapes and strides")
+    if k_cache.shape[1] == 0:
+        _fail(f"{name}: pages of no rows")
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        _fail(f"{name}: the page table must be int32 [batch, pages] with contiguous rows")
+
+
+def rope_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_length=None, slow=1.0, fast=32.0, device=None):
+    """Angles per position of each of the dim / 2 pairs, base^(-2 f / dim), and the factor the rotated values take:
+    (inv_freq fp32 [dim / 2], mscale) for ``rope`` and ``kv_append``. For contexts ``factor`` times longer than the
+    trained ``original_length``, ``scaling`` is
+      "linear": every angle divided by factor (position interpolation);
+      "base":   base grown by factor^(dim / (dim - 2)), so the slowest pair is stretched by factor and the fastest kept;
+      "ramp":   by parts (YaRN, arXiv 2309.00071): a pair that turns r times over original_length is divided by factor
+                for r < slow, kept for r > fast, mixed linearly between, and mscale = 0.1 ln(factor) + 1."""
+    if dim < 2 or dim % 2:
+        _fail(f"rope_frequencies needs an even dim (got {dim})")
+    if scaling not in (None, "linear", "base", "ramp"):
+        _fail(f"rope_frequencies: unknown scaling {scaling!r}")
+    if not base > 0 or not factor >= 1 or (scaling is None and factor != 1):
+        _fail(f"rope_frequencies: base {base}, factor {factor} with scaling {scaling!r}")
+    if scaling == "base":
+        if dim < 4:
+            _fail("rope_frequencies: base scaling needs dim of at least 4")
+        base = base * factor ** (dim / (dim - 2))
+    inv = base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    mscale = 1.0
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "ramp":
+        if not original_length or not fast > slow:
+            _fail("rope_frequencies: ramp scaling needs original_length and fast > slow")
+        turns = original_length * inv / (2 * math.pi)
+        keep = ((turns - slow) / (fast - slow)).clamp(0, 1)
+        inv = inv / factor * (1 - keep) + inv * keep
+        mscale = 0.1 * math.log(factor) + 1.0
+    return inv.to(device=device, dtype=torch.float32), mscale
+
+
+def _pairs(inv_freq, dim, name):
+    if dim < 2 or dim % 2:
+        _fail(f"{name}: head dim {dim} must be even")
+    if inv_freq is None:
+        return 0
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        _fail(f"{name}: inv_freq must be contiguous fp32 [pairs]")
+    pairs = inv_freq.shape[0]
+    if 2 * pairs > dim or pairs > MAX_ROPE_PAIRS:
+        _fail(f"{name}: {pairs} pairs do not fit a head of {dim} (at most {MAX_ROPE_PAIRS})")
+    return pairs
+
+
+def _positions(t, tokens, name):
+    if t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != tokens or not t.is_contiguous():
+        _fail(f"{name}: positions must be contiguous int64 [{tokens}] (got {t.dtype}, {tuple(t.shape)})")
+
+
+def rope(x, positions, inv_freq, interleaved=False, mscale=1.0, out=None):
+    """Rotary positions of x [tokens, heads, dim] (fp16, bf16 or fp32, any token and head strides): pair f of token t
+    turns by positions[t] * inv_freq[f]. Pairs are (f, f + len(inv_freq)), or (2f, 2f + 1) with ``interleaved``; values
+    behind the 2 len(inv_freq) rotated ones are copied. Positions int64 [tokens]; negative ones turn back (the
+    gradient of a rotation is the rotation by -positions). ``out`` may be x itself, but not overlap it otherwise."""
+    _packed(x, "rope x")
+    tokens, heads, dim = x.shape
+    pairs = _pairs(inv_freq, dim, "rope")
+    _positions(positions, tokens, "rope")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
+    else:
+        _packed(out, "rope output", x)
+        if out.shape != x.shape:
+            _fail(f"rope output has shape {tuple(out.shape)}, x {tuple(x.shape)}")
+    _one_device(x, positions, inv_freq, out)
+    _on(x, lambda: call("b2_rope", ptr(x), x.stride(0), x.stride(1), ptr(out), out.stride(0), out.stride(1), ptr(positions),
+                        ptr(inv_freq), mscale, tokens, heads, dim, pairs, int(interleaved), _DTYPE_CODES[x.dtype], stream()))
+    return out
+
+
+def kv_append(k, v, k_cache, v_cache, table, cu_q, lengths, inv_freq=None, q=None, q_out=None, positions=None,
+              interleaved=False, mscale=1.0):
+    """New keys and values k, v [tokens, kv_heads, dim] of packed sequences into a paged cache, k rotated on the way
+    (``inv_freq`` None: not), with the queries q [tokens, heads, dim] of the same tokens rotated beside them. Returns the
+    rotated queries (``q_out``, which may be q; allocated when not given), or None without q.
+
+    k_cache, v_cache [pages, page_size, kv_heads, dim] of the same dtype (fp16, bf16, fp32) and equal strides; table int32
+    [batch, pages per sequence]; cu_q int32 [batch + 1], sequence b's rows being cu_q[b] .. cu_q[b + 1]; lengths int32
+    [batch] counts the sequence's positions with the new tokens, which are the last ones. Angles use these positions, or
+    ``positions`` int64 [tokens]. Rows behind the last sequence are neither read into the cache nor written in q_out. A
+    page outside the cache or a position outside the table drops that row and sets a bit of _lib.device_status()."""
+    _packed(k, "kv_append k")
+    _packed(v, "kv_append v", k)
+    tokens, kv_heads, dim = k.shape
+    if v.shape != k.shape or kv_heads == 0:
+        _fail(f"kv_append k and v must have equal shapes [tokens, kv_heads, dim] (got {tuple(k.shape)}, {tuple(v.shape)})")
+    _cache(k_cache, v_cache, table, kv_heads, dim, k, "kv_append")
+    batch = table.shape[0]
+    _ints(cu_q, batch + 1, "kv_append cu_q")
+    _ints(lengths, batch, "kv_append lengths")
+    pairs = _pairs(inv_freq, dim, "kv_append")
+    if positions is not None:
+        _positions(positions, tokens, "kv_append")
+    heads = 0
+    if q is not None:
+        _packed(q, "kv_append q", k)
+        if q.shape[0] != tokens or q.shape[2] != dim:
+            _fail(f"kv_append q must be [{tokens}, heads, {dim}] (got {tuple(q.shape)})")
+        heads = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        else:
+            _packed(q_out, "kv_append q_out", k)
+            if q_out.shape != q.shape:
+                _fail(f"kv_append q_out has shape {tuple(q_out.shape)}, q {tuple(q.shape)}")
+    elif q_out is not None:
+        _fail("kv_append: q_out without q")
+    _one_device(k, v, k_cache, v_cache, table, cu_q, lengths, inv_freq, positions, q, q_out)
+    sq = q.stride() if heads else (0, 0)
+    so = q_out.stride() if heads else (0, 0)
+    sc = k_cache.stride()
+    _on(k, lambda: call("b2_kv_append", ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), ptr(k_cache),
+                        ptr(v_cache), sc[0], sc[1], sc[2], ptr(table), table.stride(0), table.shape[1], k_cache.shape[0],
+                        k_cache.shape[1], ptr(cu_q), ptr(lengths), batch, ptr(q), sq[0], sq[1], ptr(q_out), so[0], so[1],
+                        ptr(positions), ptr(inv_freq), mscale, tokens, heads, kv_heads, dim, pairs, int(interleaved),
+                        _DTYPE_CODES[k.dtype], stream()))
+    return q_out
+
+
+def _attn_ragged(q, k, v, table, cu_q, lengths, batch, scale, causal, softcap, window, slopes, prefix, max_q, out, lse,
+                 workspace, name):
+    """The checks and the launch that attn_paged and attn_packed share (k, v: caches, or packed rows without a table)."""
+    tokens, heads, dim = q.shape
+    kv_heads = k.shape[-2]
+    if dim not in (64, 128):
+        _fail(f"{name}: head dim {dim} (64 or 128)")
+    if kv_heads == 0 or heads == 0 or heads % kv_heads:
+        _fail(f"{name}: {heads} query heads do not group over {kv_heads} KV heads")
+    _ints(cu_q, batch + 1, f"{name} cu_q")
+    if prefix is not None:
+        _ints(prefix, batch, f"{name} prefix")
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.dim() != 1 or slopes.shape[0] != heads
+                               or not slopes.is_contiguous()):
+        _fail(f"{name} slopes must be contiguous fp32 [{heads}]")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < 3e38 or not 0 <= softcap < 3e38 or window < 0:
+        _fail(f"{name}: scale {scale} must be positive, softcap {softcap} and window {window} not negative")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    else:
+        _packed(out, f"{name} output", q)
+        if out.shape != q.shape:
+            _fail(f"{name} output has shape {tuple(out.shape)}, q {tuple(q.shape)}")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (tokens, heads) or not lse.is_contiguous()):
+        _fail(f"{name} lse must be contiguous fp32 [{tokens}, {heads}]")
+    if max_q is None:
+        max_q = -(-tokens // max(batch, 1))
+    _one_device(q, k, v, table, cu_q, lengths, prefix, slopes, out, lse, workspace)
+
+    def launch():
+        nbytes = _lib.load().b2_attn_ragged_workspace_bytes(heads, kv_heads, dim, max_q)
+        ws = workspace
+        if ws is None:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        elif not ws.is_contiguous() or ws.numel() * ws.element_size() < nbytes:
+            _fail(f"{name} workspace must be contiguous with at least {nbytes} bytes")
+        sq, so, sk = q.stride(), out.stride(), k.stride()
+        none = q.data_ptr()  # no keys at all: an empty tensor has no address, and nothing is read through this one
+        a = _lib.RaggedArgs(
+            q.data_ptr(), sq[0], sq[1], out.data_ptr(), so[0], so[1], 0 if lse is None else lse.data_ptr(),
+            k.data_ptr() or none, v.data_ptr() or none, 0 if table is None else sk[0], sk[-3], sk[-2], 0 if table is None else table.data_ptr(),
+            cu_q.data_ptr(), lengths.data_ptr(), 0 if prefix is None else prefix.data_ptr(),
+            0 if slopes is None else slopes.data_ptr(), ws.data_ptr(), 0 if table is None else table.stride(0),
+            0 if table is None else table.shape[1], k.shape[0], k.shape[1] if table is not None else 0, batch, tokens,
+            k.shape[0], heads, kv_heads, dim, _DTYPE_CODES[q.dtype], min(max_q, 1 << 30), int(causal), min(window, 1 << 30),
+            scale, softcap)
+        call("b2_attn_ragged", ctypes.byref(a), stream())
+
+    _on(q, launch)
+    return out
+
+
+def attn_paged(q, k_cache, v_cache, table, cu_q, lengths, scale=None, causal=True, softcap=0.0, window=0, slopes=None,
+               prefix=None, max_q=None, out=None, lse=None, workspace=None):
+    """Attention of packed new tokens q [tokens, heads, dim] over a paged cache that already holds their keys and values
+    (kv_append; same table, cu_q and lengths). Token i of sequence b, at position p = lengths[b] - n_b + i, sees key j
+    where (not causal or j <= p or j < prefix[b]) and (window == 0 or p - j < window). With s = scale q.k (scale
+    dim^-0.5 unless given): softcap > 0 makes it softcap tanh(s / softcap), slopes (fp32 [heads]) then subtract
+    slopes[h] |p - j|. A token that sees no key gets zeros. Rows behind the last sequence are left as they were.
+
+    fp16 or bf16, dim 64 or 128, any group of query heads per KV head, any page size; 16-byte aligned rows. ``lse``
+    (fp32 [tokens, heads]) receives log sum exp(s). ``max_q``, the new tokens of the longest sequence, chooses the kernel
+    (default: the mean). ``workspace`` (b2_attn_ragged_workspace_bytes, allocated when not given) must not be shared by
+    calls that overlap on the GPU."""
+    _packed(q, "attn_paged q", None, (torch.float16, torch.bfloat16))
+    if k_cache.dim() != 4:
+        _fail("attn_paged: k_cache must be [pages, page_size, kv_heads, dim]")
+    _cache(k_cache, v_cache, table, k_cache.shape[2], q.shape[2], q, "attn_paged")
+    _ints(lengths, table.shape[0], "attn_paged lengths")
+    return _attn_ragged(q, k_cache, v_cache, table, cu_q, lengths, table.shape[0], scale, causal, softcap, window, slopes,
+                        prefix, max_q, out, lse, workspace, "attn_paged")
+
+
+def attn_packed(q, k, v, cu_q, cu_k, scale=None, causal=True, softcap=0.0, window=0, slopes=None, prefix=None, max_q=None,
+                out=None, lse=None, workspace=None):
+    """attn_paged without a cache: sequence b's keys and values are rows cu_k[b] .. cu_k[b + 1] of k and v [keys, kv_heads,
+    dim] (equal strides), so documents packed end to end each attend inside themselves. Where a sequence has more keys
+    than queries, its queries are the last positions; the options are attn_paged's."""
+    _packed(q, "attn_packed q", None, (torch.float16, torch.bfloat16))
+    _packed(k, "attn_packed k", q)
+    _packed(v, "attn_packed v", q)
+    if k.shape != v.shape or k.stride() != v.stride() or k.shape[2] != q.shape[2]:
+        _fail("attn_packed k and v must be [keys, kv_heads, dim] with q's dim and equal shapes and strides")
+    if cu_q.dim() != 1 or cu_q.shape[0] < 1:
+        _fail("attn_packed cu_q must be int32 [batch + 1]")
+    _ints(cu_k, cu_q.shape[0], "attn_packed cu_k")
+    return _attn_ragged(q, k, v, None, cu_q, cu_k, cu_q.shape[0] - 1, scale, causal, softcap, window, slopes, prefix, max_q,
+                        out, lse, workspace, "attn_packed")
+
+
 def default_scale():
     return 1.0 / math.sqrt(HEAD_DIM)

@@ -35,6 +35,12 @@ extern "C" {
 #define B2_DEV_TIMEOUT_MMA 2u
 #define B2_DEV_TIMEOUT_EPILOGUE 4u
 #define B2_DEV_TIMEOUT_DRAIN 8u
+#define B2_DEV_BAD_PAGE 16u /* a page table entry outside the cache (or a position outside the table) was skipped */
+
+/* Element types of the entry points that take several. */
+#define B2_F16 0
+#define B2_BF16 1
+#define B2_F32 2
 
 /* Library version (major * 100 + minor). */
 int b2_version(void);
@@ -43,7 +49,7 @@ int b2_version(void);
 const char* b2_last_error(void);
 
 /* Synchronizes the current device, then returns in *flags and clears the status bits that kernels
- * set when a bounded wait ran out. Returns B2_ERR_DEVICE if any bit was set. */
+ * set when a bounded wait ran out or a page did not exist. Returns B2_ERR_DEVICE if any bit was set. */
 int b2_device_status(unsigned int* flags);
 
 /* ------------------------------------------------------------------------------------------------
@@ -254,6 +260,68 @@ int b2_attn_decode(const float* q, const float* k, const float* v, const int32_t
  * needs to start at zero. */
 int b2_attn_decode_noalloc(const float* q, const float* k, const float* v, const int32_t* lengths, float* out, int batch,
                            int heads, int kv_heads, int capacity, float scale, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Rotary positions, a paged KV cache, and attention over packed sequences (no counterpart in the reference, whose
+ * decoder keeps one fixed-capacity cache per sequence, int8_gemv.py:117-126, and reads its prompts with the text
+ * encoder's own attention).
+ *
+ * Sequences are packed: sequence b owns rows cu_q[b] .. cu_q[b + 1] of q, k, v and out (int32, ascending, on the
+ * device); rows behind cu_q[batch] are not touched. A paged cache is a pool of pages, k_cache and v_cache
+ * [num_pages, page_size, kv_heads, dim] with a contiguous last dimension and the same element strides s_page, s_row,
+ * s_head in both; position p of sequence b sits in row p % page_size of page table[b * table_ld + p / page_size].
+ * lengths[b] is the number of positions of sequence b including its new tokens, which are the last ones. cu_q, lengths,
+ * table, positions and prefix are read on the device, so a captured graph replays for other values. Table entries behind
+ * a sequence's last page are not read. A page outside [0, num_pages) that is needed, or a position outside the table, is
+ * skipped (no write; zeros read) and sets B2_DEV_BAD_PAGE; the sequence's results are then meaningless.
+ * ------------------------------------------------------------------------------------------------ */
+/* Rotary positions: out[t, h, :] is x[t, h, :] with its first 2 * pairs values rotated, pair f by the angle
+ * positions[t] * inv_freq[f] and scaled by mscale; pair f is (x[f], x[pairs + f]), or (x[2f], x[2f + 1]) when
+ * interleaved; the other values are copied. Element strides sxt, sxh (token, head) of x and sot, soh of out, the last
+ * dimension contiguous; out may be x. positions int64 (negative ones turn back), inv_freq fp32 [pairs]; dim even,
+ * 2 * pairs <= dim, pairs <= 512; dtype any of the three. */
+int b2_rope(const void* x, int64_t sxt, int64_t sxh, void* out, int64_t sot, int64_t soh, const int64_t* positions,
+            const float* inv_freq, float mscale, int tokens, int heads, int dim, int pairs, int interleaved, int dtype,
+            void* stream);
+/* New keys and values into the cache: k [tokens, kv_heads, dim] rotated as b2_rope does (pairs 0: as it is) and v as it
+ * is go to their positions lengths[b] - n_b + i; with heads > 0, q is rotated into q_out (which may be q) in the same
+ * launch. The angles use the cache positions, or positions[t] where given. */
+int b2_kv_append(const void* k, int64_t skt, int64_t skh, const void* v, int64_t svt, int64_t svh, void* k_cache,
+                 void* v_cache, int64_t s_page, int64_t s_row, int64_t s_head, const int32_t* table, int table_ld,
+                 int max_pages, int num_pages, int page_size, const int32_t* cu_q, const int32_t* lengths, int batch,
+                 const void* q, int64_t sqt, int64_t sqh, void* q_out, int64_t sot, int64_t soh, const int64_t* positions,
+                 const float* inv_freq, float mscale, int tokens, int heads, int kv_heads, int dim, int pairs,
+                 int interleaved, int dtype, void* stream);
+/* Attention of packed sequences' new tokens. Token i of sequence b sits at position pos = len - n + i of its len keys
+ * and sees key j where (not causal or j <= pos or j < prefix[b]) and (window == 0 or pos - j < window):
+ *   s = scale q.k;  s = softcap tanh(s / softcap) if softcap > 0;  s -= slopes[h] |pos - j| if slopes;
+ *   out = sum softmax(s) v;  lse = log sum exp(s)
+ * A token that sees nothing gets zeros (lse -inf). Keys are pages (table given, lengths int32 [batch]) or packed rows
+ * (table null, lengths = cu_k int32 [batch + 1], k and v [key_rows, kv_heads, dim] with strides s_row, s_head).
+ * dim 64 or 128, fp16 or bf16, heads a multiple of kv_heads; every pointer 16-byte aligned and every stride a multiple
+ * of 8 elements. max_q, an upper bound of the new tokens per sequence, chooses the kernel and nothing else. workspace:
+ * b2_attn_ragged_workspace_bytes bytes, not shared by calls that overlap on the GPU. */
+typedef struct b2_attn_ragged_args {
+    const void* q;
+    int64_t sqt, sqh;
+    void* out;
+    int64_t sot, soh;
+    float* lse; /* fp32 [tokens, heads], or null */
+    const void* k;
+    const void* v;
+    int64_t s_page, s_row, s_head;
+    const int32_t* table;
+    const int32_t* cu_q;
+    const int32_t* lengths;
+    const int32_t* prefix; /* int32 [batch], or null */
+    const float* slopes;   /* fp32 [heads], or null */
+    void* workspace;
+    int table_ld, max_pages, num_pages, page_size, batch, tokens, key_rows, heads, kv_heads, dim, dtype, max_q, causal,
+        window;
+    float scale, softcap;
+} b2_attn_ragged_args;
+int64_t b2_attn_ragged_workspace_bytes(int heads, int kv_heads, int dim, int max_q);
+int b2_attn_ragged(const b2_attn_ragged_args* args, void* stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop
