@@ -3,10 +3,15 @@
 
 using namespace b2;
 
+namespace {
+// Rows per kv head of the longest sequence that still go to the 16-row kernel.
+constexpr int64_t ROWS_LIMIT = 16;
+bool few_rows(int heads, int kv_heads, int max_q) { return (int64_t)max_q * (heads / kv_heads) <= ROWS_LIMIT; }
+}  // namespace
+
 extern "C" int64_t b2_attn_ragged_workspace_bytes(int heads, int kv_heads, int dim, int max_q) {
     if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || (dim != 64 && dim != 128)) return 0;
-    (void)max_q;
-    return rows_workspace(dim);
+    return few_rows(heads, kv_heads, max_q) ? rows_workspace(dim) : tiles_workspace(dim);
 }
 
 extern "C" int b2_attn_ragged(const b2_attn_ragged_args* p, void* stream) {
@@ -61,5 +66,6 @@ extern "C" int b2_attn_ragged(const b2_attn_ragged_args* p, void* stream) {
     a.window = p->window >= (1 << 30) ? 0 : p->window;  // no position reaches that far
     a.scale = p->scale;
     a.softcap = p->softcap;
-    return attn_rows(a, p->dim, p->dtype == B2_BF16, p->workspace, (cudaStream_t)stream);
+    auto kernel = few_rows(p->heads, p->kv_heads, p->max_q) ? attn_rows : attn_tiles;
+    return kernel(a, p->dim, p->dtype == B2_BF16, p->workspace, (cudaStream_t)stream);
 }

@@ -364,5 +364,7 @@ int launch_merge(K kernel, const RaggedArgs& a, int ctas, int rows, cudaStream_t
 // The two kernels' launchers (attn_rows.cu, attn_tiles.cu).
 int64_t rows_workspace(int dim);
 int attn_rows(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t s);
+int64_t tiles_workspace(int dim);
+int attn_tiles(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t s);
 
 }  // namespace b2

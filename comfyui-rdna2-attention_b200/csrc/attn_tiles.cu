@@ -1,0 +1,608 @@
+// Ragged attention for many rows per kv head (chunks of prompts, packed documents): 256 rows per item on tcgen05.
+//
+// With 256 rows an item does 1024 D flops per key against 4 D bytes of keys and values, well above the 250 flops per
+// byte where the tensor cores become the bound. Each CTA works on two 128-row query tiles in ping-pong: while the
+// softmax warps of one tile work on its scores, the tensor core works on the other tile (S, P and O in TMEM, P written
+// back over the consumed scores as the A operand of the second product). One CTA per SM walks its run of units
+// (attn_ragged.cuh); every barrier's phase counts on across the items.
+//
+// Keys and values are gathered by rows (cp.async, 16 bytes a lane) into the 128-byte-swizzled layout that tcgen05 reads:
+// the page table's granularity is free, and rows behind the last key are zero-filled, so nothing stale is multiplied.
+#include "attn_ragged.cuh"
+
+namespace b2 {
+namespace {
+
+__device__ unsigned int g_status;
+
+constexpr int TQ = 128, ROWS = 2 * TQ, UNIT = 128;
+constexpr int LOADERS = 3;                    // warps 0..2 load, warp 3 issues the products, warps 4..19 softmax
+constexpr int THREADS = 32 * (LOADERS + 1 + 16);
+constexpr int LIST = 48;                      // items described in shared memory at a time
+// Registers: 96 a thread at launch (640 x 96); the loading warpgroup gives 32 of its 96, the softmax warpgroups take 8
+// more each: 128 x 64 + 512 x 104 = 640 x 96.
+constexpr int REGS_LOAD = 64, REGS_SOFTMAX = 104;
+
+struct Item {
+    int q0, n, len, pos0, prefix, b, kvh, rt, unit, end, slot;  // slot -1: the item is whole
+    int64_t key0;
+};
+
+template <int D>
+struct Cfg {
+    static constexpr int TILE = 128 * D * 2;  // bytes of 128 rows (q, k or v)
+    static constexpr int OFF_Q = 0;
+    static constexpr int OFF_K = OFF_Q + 2 * TILE;
+    static constexpr int OFF_V = OFF_K + 2 * TILE;
+    static constexpr int OFF_RED = OFF_V + 2 * TILE;                           // row maxima [parity][tile][row][half]
+    static constexpr int OFF_SUM = OFF_RED + 2 * 2 * TQ * 2 * 4;               // row sums [tile][row][half]
+    static constexpr int OFF_LIST = OFF_SUM + 2 * TQ * 2 * 4;
+    static constexpr int OFF_RUN = OFF_LIST + LIST * (int)sizeof(Item);
+    static constexpr int OFF_CUR = OFF_RUN + 40 * 8;
+    static constexpr int OFF_BAR = (OFF_CUR + (int)sizeof(Cursor) + 15) / 16 * 16;
+    static constexpr int SMEM = OFF_BAR + 320 + 1024;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+    const int n = ok ? 16 : 0;  // 0 source bytes: 16 zero bytes are written
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+// Meeting point of the two softmax warps that share 32 rows (bounded).
+__device__ __forceinline__ bool pair_sync(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+    return mbar_wait(bar, parity, abort, &g_status, B2_DEV_TIMEOUT_EPILOGUE);
+}
+
+// A loading warp's copies in flight: up to three groups, each with the barrier it completes.
+struct Pending {
+    uint64_t* bar[3];
+    int n = 0;
+    __device__ __forceinline__ void pop() {
+        // The copies have landed; make them visible to the tensor core before the arrival.
+        fence_proxy_async_smem();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(bar[0]);
+        bar[0] = bar[1];
+        bar[1] = bar[2];
+        --n;
+    }
+    __device__ __forceinline__ void drain(int keep) {
+        if (n == 3 && keep < 3) {
+            asm volatile("cp.async.wait_group 2;" ::: "memory");
+            pop();
+        }
+        if (n == 2 && keep < 2) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            pop();
+        }
+        if (n == 1 && keep < 1) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            pop();
+        }
+    }
+    __device__ __forceinline__ void push(uint64_t* b) {
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (n == 0) bar[0] = b;
+        if (n == 1) bar[1] = b;
+        if (n == 2) bar[2] = b;
+        ++n;
+        drain(2);
+    }
+};
+
+// The CTA's next items into the list (one thread); returns their number, negative for the last list.
+__device__ __forceinline__ int fill_list(const RaggedArgs& a, Cursor* s_cur, Item* list) {
+    Cursor cur = *s_cur;
+    int n = 0;
+    while (cur.left > 0 && n < LIST) {
+        Item& it = list[n++];
+        const int end = (int)min((int64_t)cur.u1, cur.unit + cur.left);
+        it.q0 = cur.s.q0;
+        it.n = cur.s.n;
+        it.len = cur.s.len;
+        it.pos0 = cur.s.pos0;
+        it.prefix = cur.s.prefix;
+        it.key0 = cur.s.key0;
+        it.b = cur.b;
+        it.kvh = cur.kvh;
+        it.rt = cur.rt;
+        it.unit = cur.unit;
+        it.end = end;
+        it.slot = cur.unit == cur.u0 && end == cur.u1 ? -1 : 2 * (int)blockIdx.x + (cur.unit == cur.u0 ? 1 : 0);
+        if (cur.unit == cur.u0 && end < cur.u1)
+            a.desc[blockIdx.x] = make_int4(parts_after(cur, end), cur.b, cur.kvh, cur.rt);
+        advance<ROWS, UNIT>(a, cur, end - cur.unit);
+    }
+    *s_cur = cur;
+    return cur.left > 0 ? n : -n;
+}
+
+template <class T, int D, bool BIAS>
+__global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_constant__ RaggedArgs a) {
+    using C = Cfg<D>;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+    uint64_t* q_full = bars + 0;   // 8 arrivals: row blocks of 32
+    uint64_t* q_empty = bars + 1;
+    uint64_t* k_full = bars + 2;   // [2], 4 arrivals each
+    uint64_t* v_full = bars + 4;   // [2]
+    uint64_t* k_empty = bars + 6;  // [2]
+    uint64_t* v_empty = bars + 8;  // [2]
+    uint64_t* s_full = bars + 10;  // [2] tiles
+    uint64_t* p_full = bars + 12;  // [2]
+    uint64_t* o_done = bars + 14;  // [2]
+    uint64_t* o_free = bars + 16;  // [2]
+    uint64_t* drain = bars + 18;
+    uint64_t* pair_bar = bars + 19;  // [2 tiles][4 quarters]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 27);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* list_len = abort_flag + 1;  // items in the list; negative: the last list
+    Item* list = reinterpret_cast<Item*>(smem + C::OFF_LIST);
+
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 8);
+        mbar_init(q_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 4);
+            mbar_init(&v_full[i], 4);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 8);
+            mbar_init(&o_done[i], 1);
+            mbar_init(&o_free[i], 8);
+        }
+        mbar_init(drain, 1);
+        for (int i = 0; i < 8; ++i) mbar_init(&pair_bar[i], 2);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 3) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    // Thread 0 lists the CTA's next items; the cursor waits in shared memory meanwhile (it would cost every role's
+    // threads twenty registers).
+    Cursor* s_cur = reinterpret_cast<Cursor*>(smem + C::OFF_CUR);
+    {
+        const Cursor found = find_run<ROWS, UNIT, THREADS>(a, reinterpret_cast<int64_t*>(smem + C::OFF_RUN));
+        if (threadIdx.x == 0) {
+            *s_cur = found;
+            a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+        }
+    }
+    if (threadIdx.x == 0) *list_len = fill_list(a, s_cur, list);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    unsigned char* sQ = smem + C::OFF_Q;
+    unsigned char* sK = smem + C::OFF_K;
+    unsigned char* sV = smem + C::OFF_V;
+
+    if (warp < 4)
+        regs_dec<REGS_LOAD>();
+    else
+        regs_inc<REGS_SOFTMAX>();
+
+    // Every role walks the list, then meets the others where thread 0 writes the next one (false: there is none, or a wait
+    // ran out). Phase counters run on across items and lists.
+    auto next_list = [&](int count, bool writer) -> bool {
+        if (count <= 0) return false;
+        __syncthreads();
+        if (writer && threadIdx.x == 0) *list_len = fill_list(a, s_cur, list);
+        __syncthreads();
+        return !*abort_flag;
+    };
+    if (warp < LOADERS) {
+        uint32_t items_done = 0, units_done = 0, job = 0;
+        int count;
+        do {
+            count = *list_len;
+            const int items = abs(count);
+            Pending pend;
+            bool ok = true;
+            auto wait_free = [&](uint64_t* bar, uint32_t parity) {
+                if (mbar_try_wait(bar, parity)) return true;
+                pend.drain(0);  // what the waited-for consumer may itself be waiting for
+                return mbar_wait(bar, parity, abort_flag, &g_status, B2_DEV_TIMEOUT_PRODUCER);
+            };
+            // 32 rows of D values from the lanes' row offsets (negative: zeros) into rows 32 blk.. of a swizzled tile.
+            auto copy_rows = [&](unsigned char* tile, int blk, const T* base, int64_t off) {
+                constexpr int CH = D / 8, PASS = 32 / CH;
+                const int ch = lane % CH;
+                const uint32_t dst = smem_u32(tile) + (ch >> 3) * (128 * 128);
+#pragma unroll 4
+                for (int p = 0; p < 32 / PASS; ++p) {
+                    const int r = p * PASS + lane / CH;
+                    const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                    const int row = 32 * blk + r;
+                    cp16(dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4), base + (o < 0 ? 0 : o) + ch * 8, o >= 0);
+                }
+            };
+            for (int i = 0; i < items && ok; ++i, ++items_done) {
+                const Item& it = list[i];
+                Sequence s;
+                s.len = it.len;
+                s.key0 = it.key0;
+                const int units = it.end - it.unit;
+                const T* kh = static_cast<const T*>(a.k) + it.kvh * a.s_head;
+                const T* vh = static_cast<const T*>(a.v) + it.kvh * a.s_head;
+                auto load_tile = [&](const T* base, unsigned char* ring, uint64_t* full, uint64_t* empty, int j) {
+                    const uint32_t u = units_done + j;
+                    const int st = u & 1;
+                    bool waited = false;
+                    for (int blk = 0; blk < 4; ++blk) {
+                        if (job++ % LOADERS != (uint32_t)warp) continue;
+                        const int64_t off = key_row_offset(a, s, it.b, (it.unit + j) * UNIT + 32 * blk + lane, &g_status);
+                        if (!waited && !wait_free(&empty[st], ((u >> 1) & 1) ^ 1)) return false;
+                        waited = true;
+                        copy_rows(ring + st * C::TILE, blk, base, off);
+                        pend.push(&full[st]);
+                    }
+                    return true;
+                };
+                ok = load_tile(kh, sK, k_full, k_empty, 0);
+                if (ok) {
+                    bool waited = false;
+                    for (int blk = 0; blk < 8 && ok; ++blk) {
+                        if (job++ % LOADERS != (uint32_t)warp) continue;
+                        if (!waited) ok = wait_free(q_empty, (items_done & 1) ^ 1);
+                        waited = true;
+                        if (!ok) break;
+                        // Query rows of the item: row r is token r / group, head r % group of the kv head's group.
+                        const int r = it.rt * ROWS + 32 * blk + lane;
+                        int64_t off = -1;
+                        if (r < it.n * a.group) {
+                            const int tok = r / a.group;
+                            off = (int64_t)(it.q0 + tok) * a.sqt + (int64_t)(it.kvh * a.group + r - tok * a.group) * a.sqh;
+                        }
+                        copy_rows(sQ + (blk >> 2) * C::TILE, blk & 3, static_cast<const T*>(a.q), off);
+                        pend.push(q_full);
+                    }
+                }
+                for (int j = 0; j < units && ok; ++j) {
+                    if (j + 1 < units) ok = load_tile(kh, sK, k_full, k_empty, j + 1);
+                    if (ok) ok = load_tile(vh, sV, v_full, v_empty, j);
+                }
+                units_done += units;
+            }
+            pend.drain(0);
+        } while (next_list(count, true));
+    } else if (warp == LOADERS) {
+        uint32_t items_done = 0, units_done = 0;
+        uint32_t a_items = 0, a_units = 0, b_items = 0, b_units = 0;  // of query tile A (every item), B (items of > 128 rows)
+        int count;
+        do {
+            count = *list_len;
+            const int items = abs(count);
+            if (lane == 0) {
+                constexpr uint32_t FMT = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1 : 0;
+                constexpr uint32_t idesc_qk = idesc_make(1, FMT, 0, 0, TQ, UNIT);
+                constexpr uint32_t idesc_pv = idesc_make(1, FMT, 0, 1, TQ, D);
+                auto issue_s = [&](int t, int st) {
+                    const uint32_t k_addr = smem_u32(sK + st * C::TILE), q_addr = smem_u32(sQ + t * C::TILE);
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
+                        mma_f16_ss(tmem + t * UNIT, sdesc_sw128(q_addr + off, 16, 1024), sdesc_sw128(k_addr + off, 16, 1024),
+                                   idesc_qk, kk != 0);
+                    }
+                    tc_commit(&s_full[t]);
+                };
+                auto issue_pv = [&](int t, int st, bool first) {
+                    const uint32_t v_addr = smem_u32(sV + st * C::TILE);
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk)
+                        // P of keys [64 h, 64 h + 64) sits in columns [64 h, 64 h + 32) of the tile's S region
+                        mma_f16_ts(tmem + 256 + t * D, tmem + t * UNIT + 64 * (kk >> 2) + 8 * (kk & 3),
+                                   sdesc_sw128(v_addr + kk * 2048, 128 * 128, 1024), idesc_pv, !(first && kk == 0));
+                    tc_commit(&o_done[t]);
+                };
+                auto wait = [&](uint64_t* bar, uint32_t parity) {
+                    return mbar_wait(bar, parity, abort_flag, &g_status, B2_DEV_TIMEOUT_MMA);
+                };
+                bool ok = true;
+                for (int i = 0; i < items && ok; ++i, ++items_done) {
+                    const Item& it = list[i];
+                    const int units = it.end - it.unit;
+                    const bool two = it.n * a.group - it.rt * ROWS > TQ;
+                    uint32_t u = units_done;
+                    ok = wait(q_full, items_done & 1) && wait(&k_full[u & 1], (u >> 1) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_s(0, u & 1);
+                    if (two) issue_s(1, u & 1);
+                    tc_commit(&k_empty[u & 1]);
+                    if (units == 1) tc_commit(q_empty);
+                    for (int j = 0; j < units; ++j, ++u) {
+                        const int st = u & 1;
+                        const bool more = j + 1 < units;
+                        ok = wait(&p_full[0], (a_units + j) & 1) && wait(&v_full[st], (u >> 1) & 1);
+                        // O is free once the softmax warps have read the tile's previous item out of it
+                        if (ok && j == 0) ok = wait(&o_free[0], (a_items & 1) ^ 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_pv(0, st, j == 0);
+                        if (more) {
+                            ok = wait(&k_full[(u + 1) & 1], ((u + 1) >> 1) & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            issue_s(0, (u + 1) & 1);
+                        }
+                        if (two) {
+                            ok = wait(&p_full[1], (b_units + j) & 1);
+                            if (ok && j == 0) ok = wait(&o_free[1], (b_items & 1) ^ 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            issue_pv(1, st, j == 0);
+                        }
+                        tc_commit(&v_empty[st]);
+                        if (more) {
+                            if (two) issue_s(1, (u + 1) & 1);
+                            tc_commit(&k_empty[(u + 1) & 1]);
+                            if (j + 2 == units) tc_commit(q_empty);
+                        }
+                    }
+                    units_done += units;
+                    a_units += units;
+                    ++a_items;
+                    if (two) {
+                        b_units += units;
+                        ++b_items;
+                    }
+                }
+            }
+            __syncwarp();
+        } while (next_list(count, false));
+        if (lane == 0) {
+            tc_commit(drain);
+            if (!mbar_wait_drain(drain, 0, 100000000ull)) atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
+        }
+        __syncwarp();
+    } else {
+            // Softmax: tile t, key half hh, lane quarter (TMEM lanes 32 quarter .. + 31); thread -> query row.
+            const int sw = warp - 4;
+            const int t = sw >> 3, hh = (sw >> 2) & 1, quarter = warp & 3;
+            const int row = quarter * 32 + lane;
+            uint64_t* pbar = &pair_bar[t * 4 + quarter];
+            const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+            const uint32_t tS = tmem + lane_base + t * UNIT + 64 * hh;
+            const uint32_t tO = tmem + lane_base + 256 + t * D + (D / 2) * hh;
+            float* red = reinterpret_cast<float*>(smem + C::OFF_RED);
+            float* rl = reinterpret_cast<float*>(smem + C::OFF_SUM) + (t * TQ + row) * 2;
+            const float scale2 = a.scale * RAGGED_LOG2E;
+            const float cap2 = a.softcap * RAGGED_LOG2E, cap_in = a.softcap > 0.f ? 2.f * scale2 / a.softcap : 0.f;
+            uint32_t ucount = 0, pair_ph = 0;
+            int count;
+            do {
+            count = *list_len;
+            const int items = abs(count);
+            bool ok = true;
+            for (int i = 0; i < items && ok; ++i) {
+                const Item& it = list[i];
+                const int rows = it.n * a.group - it.rt * ROWS - t * TQ;  // valid rows of this tile
+                if (rows <= 0) continue;
+                const int units = it.end - it.unit;
+                int lo = 0, hi = 0x7fffffff, pos = 0;
+                float slope = 0.f;
+                if (row < rows) {
+                    const int r = it.rt * ROWS + t * TQ + row;
+                    const int tok = r / a.group;
+                    pos = it.pos0 + tok;
+                    hi = a.causal ? min(it.len, max(pos + 1, it.prefix)) : it.len;
+                    lo = a.window ? max(0, pos - a.window + 1) : 0;
+                    if (BIAS && a.slopes) slope = a.slopes[it.kvh * a.group + r - tok * a.group] * RAGGED_LOG2E;
+                }
+                const int lo_all = __reduce_max_sync(0xffffffffu, lo), hi_all = __reduce_min_sync(0xffffffffu, hi);
+                float m = -INFINITY, l = 0.f;
+                for (int j = 0; j < units; ++j, ++ucount) {
+                    if (!mbar_wait(&s_full[t], ucount & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const int key0 = (it.unit + j) * UNIT + 64 * hh;
+                    const bool full = key0 >= lo_all && key0 + 64 <= hi_all;
+                    // Pass 1: the half's row maximum. With a cap or a bias the finished, masked scores go back to TMEM;
+                    // without, raw scores stay and the (positive) scale is applied to the maximum.
+                    float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32_wait(tS + c * 32, v);
+                        if (BIAS) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const float raw = __uint_as_float(v[e]);
+                                float y = raw * scale2;
+                                if (a.softcap > 0.f) y = capped(raw * cap_in, cap2);
+                                const int key = key0 + c * 32 + e;
+                                y = fmaf(-slope, (float)abs(pos - key), y);
+                                if (!full && (key < lo || key >= hi)) y = -INFINITY;
+                                v[e] = __float_as_uint(y);
+                            }
+                            tmem_st32(tS + c * 32, v);
+                        }
+                        if (BIAS || full) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                                for (int q = 0; q < 4; ++q)
+                                    mm[q] = max3(mm[q], __uint_as_float(v[e + 2 * q]), __uint_as_float(v[e + 2 * q + 1]));
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const int key = key0 + c * 32 + e;
+                                if (key >= lo && key < hi) mm[e & 3] = fmaxf(mm[e & 3], __uint_as_float(v[e]));
+                            }
+                        }
+                    }
+                    if (BIAS) tmem_wait_st();
+                    // The two halves' maxima meet (slot by parity, so a fast warp never overwrites a slot its partner
+                    // still reads), and both take the same rescale decision: the maximum moves only when a row's grew by
+                    // more than 2^8, so p stays below 2^8 (inside fp16) and O is rescaled rarely.
+                    float* rm = red + (((ucount & 1) * 2 + t) * TQ + row) * 2;
+                    rm[hh] = max3(mm[0], mm[1], fmaxf(mm[2], mm[3]));
+                    if (!pair_sync(pbar, pair_ph++ & 1, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    float mx = fmaxf(rm[0], rm[1]);
+                    if (!BIAS) mx *= scale2;
+                    if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+                        const float mn = fmaxf(m, mx);
+                        const float alpha = m == -INFINITY ? 0.f : ex2_approx(m - mn);
+                        m = mn;
+                        l *= alpha;
+                        if (j > 0) {
+                            // O holds the products of the previous units; they must be complete before the rescale.
+                            if (!mbar_wait(&o_done[t], (ucount - 1) & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D / 64; ++c) {
+                                uint32_t o[32];
+                                tmem_ld32_wait(tO + c * 32, o);
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                                tmem_st32(tO + c * 32, o);
+                            }
+                        }
+                    }
+                    // Pass 2: p = 2^(s - m); l sums the fp32 p; P, rounded to the inputs' type (half a step per key,
+                    // averaged over the row), goes into the columns already read: 32 scores -> 16 columns.
+                    const uint64_t c2 = BIAS ? pk2(1.f, 1.f) : pk2(scale2, scale2);
+                    const float nm = m == -INFINITY ? 0.f : -m;
+                    const uint64_t nm2 = pk2(nm, nm);
+                    uint64_t l2 = pk2(0.f, 0.f);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t v[32], pk[16];
+                        tmem_ld32_wait(tS + c * 32, v);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int key = key0 + c * 32 + 2 * e;
+                            const float2 x = upk2(fma2(pk2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, nm2));
+                            float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
+                            if (!BIAS && !full) {
+                                if (key < lo || key >= hi) p0 = 0.f;
+                                if (key + 1 < lo || key + 1 >= hi) p1 = 0.f;
+                            }
+                            l2 = add2(l2, pk2(p0, p1));
+                            pk[e] = Pair<T>::pack(p0, p1);
+                        }
+                        tmem_st16(tS + c * 16, pk);
+                    }
+                    const float2 lf = upk2(l2);
+                    l += lf.x + lf.y;
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[t]);
+                }
+                if (!ok) break;
+                // The row sum is the two halves' sums (half 0 first in both warps).
+                rl[hh] = l;
+                if (!pair_sync(pbar, pair_ph++ & 1, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                l = rl[0] + rl[1];
+                if (!mbar_wait(&o_done[t], (ucount - 1) & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const bool live = row < rows;
+                const int r = it.rt * ROWS + t * TQ + row;
+                const int tok = it.q0 + r / a.group, head = it.kvh * a.group + r % a.group;
+                if (it.slot < 0) {
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    T* dst = static_cast<T*>(a.out) + (int64_t)tok * a.sot + (int64_t)head * a.soh + (D / 2) * hh;
+#pragma unroll 1
+                    for (int c = 0; c < D / 64; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32_wait(tO + c * 32, o);
+                        if (live) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                uint32_t u[4];
+#pragma unroll
+                                for (int z = 0; z < 4; ++z)
+                                    u[z] = Pair<T>::pack(__uint_as_float(o[8 * e + 2 * z]) * inv,
+                                                         __uint_as_float(o[8 * e + 2 * z + 1]) * inv);
+                                *reinterpret_cast<uint4*>(dst + c * 32 + 8 * e) = make_uint4(u[0], u[1], u[2], u[3]);
+                            }
+                        }
+                    }
+                    if (a.lse && live && hh == 0) a.lse[(int64_t)tok * a.heads + head] = log_sum(m, l);
+                } else {
+                    const int64_t srow = (int64_t)it.slot * ROWS + t * TQ + row;
+                    float* dst = a.part_o + srow * D + (D / 2) * hh;
+#pragma unroll 1
+                    for (int c = 0; c < D / 64; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32_wait(tO + c * 32, o);
+                        if (live) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                *reinterpret_cast<uint4*>(dst + c * 32 + 4 * e) =
+                                    make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        }
+                    }
+                    if (live && hh == 0) a.part_ml[srow] = make_float2(m, l);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&o_free[t]);
+            }
+            } while (next_list(count, false));
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == LOADERS) tmem_dealloc(tmem, 512);
+}
+
+template <class T, int D, bool BIAS>
+int launch_tiles(const RaggedArgs& a, cudaStream_t s) {
+    if (int rc = set_smem(attn_tiles_kernel<T, D, BIAS>, Cfg<D>::SMEM)) return rc;
+    const int ctas = sm_count();
+    attn_tiles_kernel<T, D, BIAS><<<ctas, THREADS, Cfg<D>::SMEM, s>>>(a);
+    if (int rc = check_launch("attn_tiles_kernel")) return rc;
+    return launch_merge(merge_kernel<T, D, ROWS>, a, ctas, ROWS, s);
+}
+
+}  // namespace
+
+int64_t tiles_workspace(int dim) { return ragged_workspace(sm_count(), ROWS, dim); }
+
+int attn_tiles(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t s) {
+    const bool bias = a.softcap > 0.f || a.slopes;
+    ragged_slots(a, workspace, sm_count(), ROWS, dim);
+#define B2_TILES(T, D) return bias ? launch_tiles<T, D, true>(a, s) : launch_tiles<T, D, false>(a, s)
+    if (dim == 128) {
+        if (bf16) B2_TILES(__nv_bfloat16, 128);
+        B2_TILES(__half, 128);
+    }
+    if (bf16) B2_TILES(__nv_bfloat16, 64);
+    B2_TILES(__half, 64);
+#undef B2_TILES
+}
+
+unsigned int read_status_attn_tiles() {
+    unsigned int v = 0, zero = 0;
+    cudaMemcpyFromSymbol(&v, g_status, sizeof(v));
+    if (v) cudaMemcpyToSymbol(g_status, &zero, sizeof(zero));
+    return v;
+}
+
+}  // namespace b2

@@ -87,7 +87,7 @@ int b2_device_status(unsigned int* flags) {
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return b2::fail(B2_ERR_CUDA, "cudaDeviceSynchronize: %s", cudaGetErrorString(e));
     unsigned int f = b2::read_status_gemm() | b2::read_status_attention() | b2::read_status_gemm_w4a8() |
-                     b2::read_status_rope() | b2::read_status_attn_rows();
+                     b2::read_status_rope() | b2::read_status_attn_rows() | b2::read_status_attn_tiles();
     if (flags) *flags = f;
     if (f) return b2::fail(B2_ERR_DEVICE, "device status 0x%x: %s", f,
                               f == B2_DEV_BAD_PAGE ? "a page table entry outside the cache" : "a bounded wait ran out");

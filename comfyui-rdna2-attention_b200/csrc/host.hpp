@@ -55,5 +55,6 @@ unsigned int read_status_attention();
 unsigned int read_status_gemm_w4a8();
 unsigned int read_status_rope();
 unsigned int read_status_attn_rows();
+unsigned int read_status_attn_tiles();
 
 }  // namespace b2
