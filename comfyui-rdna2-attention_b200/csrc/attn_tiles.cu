@@ -16,12 +16,12 @@ namespace {
 __device__ unsigned int g_status;
 
 constexpr int TQ = 128, ROWS = 2 * TQ, UNIT = 128;
-constexpr int LOADERS = 3;                    // warps 0..2 load, warp 3 issues the products, warps 4..19 softmax
-constexpr int THREADS = 32 * (LOADERS + 1 + 16);
+constexpr int LOADERS = 3, MMA_WARP = 11;      // warps 0..7 softmax, 8..10 load, 11 issues the products
+constexpr int THREADS = 384, LIST_WRITER = 8 * 32;
 constexpr int LIST = 48;                      // items described in shared memory at a time
-// Registers: 96 a thread at launch (640 x 96); the loading warpgroup gives 32 of its 96, the softmax warpgroups take 8
-// more each: 128 x 64 + 512 x 104 = 640 x 96.
-constexpr int REGS_LOAD = 64, REGS_SOFTMAX = 104;
+// Registers: 168 a thread at launch; the loading warpgroup keeps 80, the two softmax warpgroups take 208:
+// 128 x 80 + 256 x 208 = 63488 of the launch's 384 x 168 = 64512.
+constexpr int REGS_LOAD = 80, REGS_SOFTMAX = 208;
 
 struct Item {
     int q0, n, len, pos0, prefix, b, kvh, rt, unit, end, slot;  // slot -1: the item is whole
@@ -34,25 +34,16 @@ struct Cfg {
     static constexpr int OFF_Q = 0;
     static constexpr int OFF_K = OFF_Q + 2 * TILE;
     static constexpr int OFF_V = OFF_K + 2 * TILE;
-    static constexpr int OFF_RED = OFF_V + 2 * TILE;                           // row maxima [parity][tile][row][half]
-    static constexpr int OFF_SUM = OFF_RED + 2 * 2 * TQ * 2 * 4;               // row sums [tile][row][half]
-    static constexpr int OFF_LIST = OFF_SUM + 2 * TQ * 2 * 4;
+    static constexpr int OFF_LIST = OFF_V + 2 * TILE;
     static constexpr int OFF_RUN = OFF_LIST + LIST * (int)sizeof(Item);
     static constexpr int OFF_CUR = OFF_RUN + 40 * 8;
     static constexpr int OFF_BAR = (OFF_CUR + (int)sizeof(Cursor) + 15) / 16 * 16;
-    static constexpr int SMEM = OFF_BAR + 320 + 1024;
+    static constexpr int SMEM = OFF_BAR + 256 + 1024;
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
     const int n = ok ? 16 : 0;  // 0 source bytes: 16 zero bytes are written
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-
-// Meeting point of the two softmax warps that share 32 rows (bounded).
-__device__ __forceinline__ bool pair_sync(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-    return mbar_wait(bar, parity, abort, &g_status, B2_DEV_TIMEOUT_EPILOGUE);
 }
 
 // A loading warp's copies in flight: up to three groups, each with the barrier it completes.
@@ -132,12 +123,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
     uint64_t* k_empty = bars + 6;  // [2]
     uint64_t* v_empty = bars + 8;  // [2]
     uint64_t* s_full = bars + 10;  // [2] tiles
-    uint64_t* p_full = bars + 12;  // [2]
-    uint64_t* o_done = bars + 14;  // [2]
-    uint64_t* o_free = bars + 16;  // [2]
-    uint64_t* drain = bars + 18;
-    uint64_t* pair_bar = bars + 19;  // [2 tiles][4 quarters]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 27);
+    uint64_t* p_half = bars + 12;  // [2] keys 0..63 of P
+    uint64_t* p_full = bars + 14;  // [2]
+    uint64_t* o_done = bars + 16;  // [2]
+    uint64_t* o_free = bars + 18;  // [2]
+    uint64_t* drain = bars + 20;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* list_len = abort_flag + 1;  // items in the list; negative: the last list
     Item* list = reinterpret_cast<Item*>(smem + C::OFF_LIST);
@@ -153,16 +144,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 8);
+            mbar_init(&p_half[i], 4);  // one arrival per softmax warp of the tile
+            mbar_init(&p_full[i], 4);
             mbar_init(&o_done[i], 1);
-            mbar_init(&o_free[i], 8);
+            mbar_init(&o_free[i], 4);
         }
         mbar_init(drain, 1);
-        for (int i = 0; i < 8; ++i) mbar_init(&pair_bar[i], 2);
         *abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 3) {
+    if (warp == MMA_WARP) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -185,73 +176,72 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
     unsigned char* sK = smem + C::OFF_K;
     unsigned char* sV = smem + C::OFF_V;
 
-    if (warp < 4)
-        regs_dec<REGS_LOAD>();
-    else
-        regs_inc<REGS_SOFTMAX>();
-
-    // Every role walks the list, then meets the others where thread 0 writes the next one (false: there is none, or a wait
-    // ran out). Phase counters run on across items and lists.
+    // Every role walks the list, then meets the others where thread LIST_WRITER writes the next one (false: there is none,
+    // or a wait ran out). Phase counters run on across items and lists.
     auto next_list = [&](int count, bool writer) -> bool {
         if (count <= 0) return false;
         __syncthreads();
-        if (writer && threadIdx.x == 0) *list_len = fill_list(a, s_cur, list);
+        if (writer && threadIdx.x == LIST_WRITER) *list_len = fill_list(a, s_cur, list);
         __syncthreads();
         return !*abort_flag;
     };
-    if (warp < LOADERS) {
-        uint32_t items_done = 0, units_done = 0, job = 0;
-        int count;
-        do {
-            count = *list_len;
-            const int items = abs(count);
-            Pending pend;
-            bool ok = true;
-            auto wait_free = [&](uint64_t* bar, uint32_t parity) {
-                if (mbar_try_wait(bar, parity)) return true;
-                pend.drain(0);  // what the waited-for consumer may itself be waiting for
-                return mbar_wait(bar, parity, abort_flag, &g_status, B2_DEV_TIMEOUT_PRODUCER);
-            };
-            // 32 rows of D values from the lanes' row offsets (negative: zeros) into rows 32 blk.. of a swizzled tile.
-            auto copy_rows = [&](unsigned char* tile, int blk, const T* base, int64_t off) {
-                constexpr int CH = D / 8, PASS = 32 / CH;
-                const int ch = lane % CH;
-                const uint32_t dst = smem_u32(tile) + (ch >> 3) * (128 * 128);
-#pragma unroll 4
-                for (int p = 0; p < 32 / PASS; ++p) {
-                    const int r = p * PASS + lane / CH;
-                    const int64_t o = __shfl_sync(0xffffffffu, off, r);
-                    const int row = 32 * blk + r;
-                    cp16(dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4), base + (o < 0 ? 0 : o) + ch * 8, o >= 0);
-                }
-            };
-            for (int i = 0; i < items && ok; ++i, ++items_done) {
-                const Item& it = list[i];
-                Sequence s;
-                s.len = it.len;
-                s.key0 = it.key0;
-                const int units = it.end - it.unit;
-                const T* kh = static_cast<const T*>(a.k) + it.kvh * a.s_head;
-                const T* vh = static_cast<const T*>(a.v) + it.kvh * a.s_head;
-                auto load_tile = [&](const T* base, unsigned char* ring, uint64_t* full, uint64_t* empty, int j) {
-                    const uint32_t u = units_done + j;
-                    const int st = u & 1;
-                    bool waited = false;
-                    for (int blk = 0; blk < 4; ++blk) {
-                        if (job++ % LOADERS != (uint32_t)warp) continue;
-                        const int64_t off = key_row_offset(a, s, it.b, (it.unit + j) * UNIT + 32 * blk + lane, &g_status);
-                        if (!waited && !wait_free(&empty[st], ((u >> 1) & 1) ^ 1)) return false;
-                        waited = true;
-                        copy_rows(ring + st * C::TILE, blk, base, off);
-                        pend.push(&full[st]);
-                    }
-                    return true;
+
+    if (warp >= 8) {
+        // Each role's code stands in the branch of its own register budget: behind a join the smaller one would hold.
+        regs_dec<REGS_LOAD>();
+        if (warp < 8 + LOADERS) {
+            const uint32_t loader = warp - 8;
+            uint32_t items_done = 0, units_done = 0, job = 0;
+            int count;
+            do {
+                count = *list_len;
+                const int items = abs(count);
+                Pending pend;
+                bool ok = true;
+                auto wait_free = [&](uint64_t* bar, uint32_t parity) {
+                    if (mbar_try_wait(bar, parity)) return true;
+                    pend.drain(0);  // what the waited-for consumer may itself be waiting for
+                    return mbar_wait(bar, parity, abort_flag, &g_status, B2_DEV_TIMEOUT_PRODUCER);
                 };
-                ok = load_tile(kh, sK, k_full, k_empty, 0);
-                if (ok) {
+                // 32 rows of D values from the lanes' row offsets (negative: zeros) into rows 32 blk.. of a swizzled tile.
+                auto copy_rows = [&](unsigned char* tile, int blk, const T* base, int64_t off) {
+                    constexpr int CH = D / 8, PASS = 32 / CH;
+                    const int ch = lane % CH;
+                    const uint32_t dst = smem_u32(tile) + (ch >> 3) * (128 * 128);
+#pragma unroll 8
+                    for (int p = 0; p < 32 / PASS; ++p) {
+                        const int r = p * PASS + lane / CH;
+                        const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                        const int row = 32 * blk + r;
+                        cp16(dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4), base + (o < 0 ? 0 : o) + ch * 8, o >= 0);
+                    }
+                };
+                for (int i = 0; i < items && ok; ++i, ++items_done) {
+                    const Item& it = list[i];
+                    Sequence s;
+                    s.len = it.len;
+                    s.key0 = it.key0;
+                    const int units = it.end - it.unit, first = it.unit, b = it.b;
+                    const T* kh = static_cast<const T*>(a.k) + it.kvh * a.s_head;
+                    const T* vh = static_cast<const T*>(a.v) + it.kvh * a.s_head;
+                    auto load_tile = [&](const T* base, unsigned char* ring, uint64_t* full, uint64_t* empty, int j) {
+                        const uint32_t u = units_done + j;
+                        const int st = u & 1;
+                        bool waited = false;
+                        for (int blk = 0; blk < 4; ++blk) {
+                            if (job++ % LOADERS != loader) continue;
+                            const int64_t off = key_row_offset(a, s, b, (first + j) * UNIT + 32 * blk + lane, &g_status);
+                            if (!waited && !wait_free(&empty[st], ((u >> 1) & 1) ^ 1)) return false;
+                            waited = true;
+                            copy_rows(ring + st * C::TILE, blk, base, off);
+                            pend.push(&full[st]);
+                        }
+                        return true;
+                    };
+                    ok = load_tile(kh, sK, k_full, k_empty, 0);
                     bool waited = false;
                     for (int blk = 0; blk < 8 && ok; ++blk) {
-                        if (job++ % LOADERS != (uint32_t)warp) continue;
+                        if (job++ % LOADERS != loader) continue;
                         if (!waited) ok = wait_free(q_empty, (items_done & 1) ^ 1);
                         waited = true;
                         if (!ok) break;
@@ -265,130 +255,124 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                         copy_rows(sQ + (blk >> 2) * C::TILE, blk & 3, static_cast<const T*>(a.q), off);
                         pend.push(q_full);
                     }
+                    for (int j = 0; j < units && ok; ++j) {
+                        if (j + 1 < units) ok = load_tile(kh, sK, k_full, k_empty, j + 1);
+                        if (ok) ok = load_tile(vh, sV, v_full, v_empty, j);
+                    }
+                    units_done += units;
                 }
-                for (int j = 0; j < units && ok; ++j) {
-                    if (j + 1 < units) ok = load_tile(kh, sK, k_full, k_empty, j + 1);
-                    if (ok) ok = load_tile(vh, sV, v_full, v_empty, j);
+                pend.drain(0);
+            } while (next_list(count, true));
+        } else {
+            uint32_t items_done = 0, units_done = 0;
+            uint32_t tile_items[2] = {0, 0}, tile_units[2] = {0, 0};  // of query tile A (every item), B (items of > 128 rows)
+            int count;
+            do {
+                count = *list_len;
+                const int items = abs(count);
+                if (lane == 0) {
+                    constexpr uint32_t FMT = __is_same(T, __nv_bfloat16) ? 1 : 0;
+                    constexpr uint32_t idesc_qk = idesc_make(1, FMT, 0, 0, TQ, UNIT);
+                    constexpr uint32_t idesc_pv = idesc_make(1, FMT, 0, 1, TQ, D);
+                    auto wait = [&](uint64_t* bar, uint32_t parity) {
+                        return mbar_wait(bar, parity, abort_flag, &g_status, B2_DEV_TIMEOUT_MMA);
+                    };
+                    auto issue_s = [&](int t, int st) {
+                        const uint32_t k_addr = smem_u32(sK + st * C::TILE), q_addr = smem_u32(sQ + t * C::TILE);
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
+                            mma_f16_ss(tmem + t * UNIT, sdesc_sw128(q_addr + off, 16, 1024), sdesc_sw128(k_addr + off, 16, 1024),
+                                       idesc_qk, kk != 0);
+                        }
+                        tc_commit(&s_full[t]);
+                    };
+                    // O of tile t += P V for unit j of the item: the first 64 keys as soon as their P is there.
+                    auto issue_pv = [&](int t, int st, int j) {
+                        const uint32_t v_addr = smem_u32(sV + st * C::TILE);
+                        const uint32_t ph = (tile_units[t] + j) & 1;
+                        if (!wait(&p_half[t], ph)) return false;
+                        // O is free once the softmax warps have read the tile's previous item out of it
+                        if (j == 0 && !wait(&o_free[t], (tile_items[t] & 1) ^ 1)) return false;
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk) {
+                            if (kk == 4) {
+                                if (!wait(&p_full[t], ph)) return false;
+                                tc_fence_after();
+                            }
+                            mma_f16_ts(tmem + 256 + t * D, tmem + t * UNIT + 8 * kk, sdesc_sw128(v_addr + kk * 2048, 128 * 128, 1024),
+                                       idesc_pv, (j | kk) != 0);
+                        }
+                        tc_commit(&o_done[t]);
+                        return true;
+                    };
+                    bool ok = true;
+                    for (int i = 0; i < items && ok; ++i, ++items_done) {
+                        const Item& it = list[i];
+                        const int units = it.end - it.unit;
+                        const bool two = it.n * a.group - it.rt * ROWS > TQ;
+                        uint32_t u = units_done;
+                        ok = wait(q_full, items_done & 1) && wait(&k_full[u & 1], (u >> 1) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_s(0, u & 1);
+                        if (two) issue_s(1, u & 1);
+                        tc_commit(&k_empty[u & 1]);
+                        if (units == 1) tc_commit(q_empty);
+                        for (int j = 0; j < units; ++j, ++u) {
+                            const int st = u & 1, nx = (u + 1) & 1;
+                            const bool more = j + 1 < units;
+                            ok = wait(&v_full[st], (u >> 1) & 1) && issue_pv(0, st, j);
+                            if (ok && more) {
+                                ok = wait(&k_full[nx], ((u + 1) >> 1) & 1);
+                                if (ok) {
+                                    tc_fence_after();
+                                    issue_s(0, nx);
+                                }
+                            }
+                            if (ok && two) ok = issue_pv(1, st, j);
+                            if (!ok) break;
+                            tc_commit(&v_empty[st]);
+                            if (more) {
+                                if (two) issue_s(1, nx);
+                                tc_commit(&k_empty[nx]);
+                                if (j + 2 == units) tc_commit(q_empty);
+                            }
+                        }
+                        units_done += units;
+                        for (int t = 0; t <= (two ? 1 : 0); ++t) {
+                            tile_units[t] += units;
+                            ++tile_items[t];
+                        }
+                    }
                 }
-                units_done += units;
+                __syncwarp();
+            } while (next_list(count, false));
+            if (lane == 0) {
+                tc_commit(drain);
+                if (!mbar_wait_drain(drain, 0, 100000000ull)) atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
             }
-            pend.drain(0);
-        } while (next_list(count, true));
-    } else if (warp == LOADERS) {
-        uint32_t items_done = 0, units_done = 0;
-        uint32_t a_items = 0, a_units = 0, b_items = 0, b_units = 0;  // of query tile A (every item), B (items of > 128 rows)
+            __syncwarp();
+        }
+    } else {
+        regs_inc<REGS_SOFTMAX>();
+        // Softmax: warps 0..3 tile A, 4..7 tile B; thread -> query row (TMEM lane), its 128 scores of a unit in registers.
+        const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tS = tmem + lane_base + t * UNIT, tO = tmem + lane_base + 256 + t * D;
+        const float scale2 = a.scale * RAGGED_LOG2E;
+        const float cap2 = a.softcap * RAGGED_LOG2E, cap_in = a.softcap > 0.f ? 2.f * scale2 / a.softcap : 0.f;
+        uint32_t ucount = 0;
         int count;
         do {
             count = *list_len;
             const int items = abs(count);
-            if (lane == 0) {
-                constexpr uint32_t FMT = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1 : 0;
-                constexpr uint32_t idesc_qk = idesc_make(1, FMT, 0, 0, TQ, UNIT);
-                constexpr uint32_t idesc_pv = idesc_make(1, FMT, 0, 1, TQ, D);
-                auto issue_s = [&](int t, int st) {
-                    const uint32_t k_addr = smem_u32(sK + st * C::TILE), q_addr = smem_u32(sQ + t * C::TILE);
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
-                        mma_f16_ss(tmem + t * UNIT, sdesc_sw128(q_addr + off, 16, 1024), sdesc_sw128(k_addr + off, 16, 1024),
-                                   idesc_qk, kk != 0);
-                    }
-                    tc_commit(&s_full[t]);
-                };
-                auto issue_pv = [&](int t, int st, bool first) {
-                    const uint32_t v_addr = smem_u32(sV + st * C::TILE);
-#pragma unroll
-                    for (int kk = 0; kk < 8; ++kk)
-                        // P of keys [64 h, 64 h + 64) sits in columns [64 h, 64 h + 32) of the tile's S region
-                        mma_f16_ts(tmem + 256 + t * D, tmem + t * UNIT + 64 * (kk >> 2) + 8 * (kk & 3),
-                                   sdesc_sw128(v_addr + kk * 2048, 128 * 128, 1024), idesc_pv, !(first && kk == 0));
-                    tc_commit(&o_done[t]);
-                };
-                auto wait = [&](uint64_t* bar, uint32_t parity) {
-                    return mbar_wait(bar, parity, abort_flag, &g_status, B2_DEV_TIMEOUT_MMA);
-                };
-                bool ok = true;
-                for (int i = 0; i < items && ok; ++i, ++items_done) {
-                    const Item& it = list[i];
-                    const int units = it.end - it.unit;
-                    const bool two = it.n * a.group - it.rt * ROWS > TQ;
-                    uint32_t u = units_done;
-                    ok = wait(q_full, items_done & 1) && wait(&k_full[u & 1], (u >> 1) & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    issue_s(0, u & 1);
-                    if (two) issue_s(1, u & 1);
-                    tc_commit(&k_empty[u & 1]);
-                    if (units == 1) tc_commit(q_empty);
-                    for (int j = 0; j < units; ++j, ++u) {
-                        const int st = u & 1;
-                        const bool more = j + 1 < units;
-                        ok = wait(&p_full[0], (a_units + j) & 1) && wait(&v_full[st], (u >> 1) & 1);
-                        // O is free once the softmax warps have read the tile's previous item out of it
-                        if (ok && j == 0) ok = wait(&o_free[0], (a_items & 1) ^ 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        issue_pv(0, st, j == 0);
-                        if (more) {
-                            ok = wait(&k_full[(u + 1) & 1], ((u + 1) >> 1) & 1);
-                            if (!ok) break;
-                            tc_fence_after();
-                            issue_s(0, (u + 1) & 1);
-                        }
-                        if (two) {
-                            ok = wait(&p_full[1], (b_units + j) & 1);
-                            if (ok && j == 0) ok = wait(&o_free[1], (b_items & 1) ^ 1);
-                            if (!ok) break;
-                            tc_fence_after();
-                            issue_pv(1, st, j == 0);
-                        }
-                        tc_commit(&v_empty[st]);
-                        if (more) {
-                            if (two) issue_s(1, (u + 1) & 1);
-                            tc_commit(&k_empty[(u + 1) & 1]);
-                            if (j + 2 == units) tc_commit(q_empty);
-                        }
-                    }
-                    units_done += units;
-                    a_units += units;
-                    ++a_items;
-                    if (two) {
-                        b_units += units;
-                        ++b_items;
-                    }
-                }
-            }
-            __syncwarp();
-        } while (next_list(count, false));
-        if (lane == 0) {
-            tc_commit(drain);
-            if (!mbar_wait_drain(drain, 0, 100000000ull)) atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
-        }
-        __syncwarp();
-    } else {
-            // Softmax: tile t, key half hh, lane quarter (TMEM lanes 32 quarter .. + 31); thread -> query row.
-            const int sw = warp - 4;
-            const int t = sw >> 3, hh = (sw >> 2) & 1, quarter = warp & 3;
-            const int row = quarter * 32 + lane;
-            uint64_t* pbar = &pair_bar[t * 4 + quarter];
-            const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-            const uint32_t tS = tmem + lane_base + t * UNIT + 64 * hh;
-            const uint32_t tO = tmem + lane_base + 256 + t * D + (D / 2) * hh;
-            float* red = reinterpret_cast<float*>(smem + C::OFF_RED);
-            float* rl = reinterpret_cast<float*>(smem + C::OFF_SUM) + (t * TQ + row) * 2;
-            const float scale2 = a.scale * RAGGED_LOG2E;
-            const float cap2 = a.softcap * RAGGED_LOG2E, cap_in = a.softcap > 0.f ? 2.f * scale2 / a.softcap : 0.f;
-            uint32_t ucount = 0, pair_ph = 0;
-            int count;
-            do {
-            count = *list_len;
-            const int items = abs(count);
-            bool ok = true;
-            for (int i = 0; i < items && ok; ++i) {
+            for (int i = 0; i < items; ++i) {
                 const Item& it = list[i];
                 const int rows = it.n * a.group - it.rt * ROWS - t * TQ;  // valid rows of this tile
                 if (rows <= 0) continue;
-                const int units = it.end - it.unit;
+                const int first = it.unit, units = it.end - it.unit;
                 int lo = 0, hi = 0x7fffffff, pos = 0;
                 float slope = 0.f;
                 if (row < rows) {
@@ -401,60 +385,42 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                 }
                 const int lo_all = __reduce_max_sync(0xffffffffu, lo), hi_all = __reduce_min_sync(0xffffffffu, hi);
                 float m = -INFINITY, l = 0.f;
+                bool ok = true;
                 for (int j = 0; j < units; ++j, ++ucount) {
                     if (!mbar_wait(&s_full[t], ucount & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const int key0 = (it.unit + j) * UNIT + 64 * hh;
-                    const bool full = key0 >= lo_all && key0 + 64 <= hi_all;
-                    // Pass 1: the half's row maximum. With a cap or a bias the finished, masked scores go back to TMEM;
-                    // without, raw scores stay and the (positive) scale is applied to the maximum.
+                    uint32_t v[128];
+                    tmem_ld128_wait(tS, v);
+                    const int key0 = (first + j) * UNIT;
+                    if (BIAS) {
+                        // finished scores in the base-2 domain
+#pragma unroll
+                        for (int e = 0; e < 128; ++e) {
+                            const float raw = __uint_as_float(v[e]);
+                            float y = raw * scale2;
+                            if (a.softcap > 0.f) y = capped(raw * cap_in, cap2);
+                            v[e] = __float_as_uint(fmaf(-slope, (float)abs(pos - key0 - e), y));
+                        }
+                    }
+                    if (key0 < lo_all || key0 + UNIT > hi_all) {
+                        const int l0 = lo - key0, h0 = hi - key0;
+#pragma unroll
+                        for (int e = 0; e < 128; ++e)
+                            if (e < l0 || e >= h0) v[e] = 0xff800000u;  // -inf
+                    }
                     float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32_wait(tS + c * 32, v);
-                        if (BIAS) {
+                    for (int e = 0; e < 128; e += 8)
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const float raw = __uint_as_float(v[e]);
-                                float y = raw * scale2;
-                                if (a.softcap > 0.f) y = capped(raw * cap_in, cap2);
-                                const int key = key0 + c * 32 + e;
-                                y = fmaf(-slope, (float)abs(pos - key), y);
-                                if (!full && (key < lo || key >= hi)) y = -INFINITY;
-                                v[e] = __float_as_uint(y);
-                            }
-                            tmem_st32(tS + c * 32, v);
-                        }
-                        if (BIAS || full) {
-#pragma unroll
-                            for (int e = 0; e < 32; e += 8)
-#pragma unroll
-                                for (int q = 0; q < 4; ++q)
-                                    mm[q] = max3(mm[q], __uint_as_float(v[e + 2 * q]), __uint_as_float(v[e + 2 * q + 1]));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const int key = key0 + c * 32 + e;
-                                if (key >= lo && key < hi) mm[e & 3] = fmaxf(mm[e & 3], __uint_as_float(v[e]));
-                            }
-                        }
-                    }
-                    if (BIAS) tmem_wait_st();
-                    // The two halves' maxima meet (slot by parity, so a fast warp never overwrites a slot its partner
-                    // still reads), and both take the same rescale decision: the maximum moves only when a row's grew by
-                    // more than 2^8, so p stays below 2^8 (inside fp16) and O is rescaled rarely.
-                    float* rm = red + (((ucount & 1) * 2 + t) * TQ + row) * 2;
-                    rm[hh] = max3(mm[0], mm[1], fmaxf(mm[2], mm[3]));
-                    if (!pair_sync(pbar, pair_ph++ & 1, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    float mx = fmaxf(rm[0], rm[1]);
-                    if (!BIAS) mx *= scale2;
+                        for (int q = 0; q < 4; ++q)
+                            mm[q] = max3(mm[q], __uint_as_float(v[e + 2 * q]), __uint_as_float(v[e + 2 * q + 1]));
+                    float mx = max3(mm[0], mm[1], fmaxf(mm[2], mm[3]));
+                    if (!BIAS) mx *= scale2;  // scale2 > 0
+                    // The maximum moves only when a row's grew by more than 2^8: p stays below 2^8 (inside fp16) and O is
+                    // rescaled rarely.
                     if (__any_sync(0xffffffffu, mx > m + 8.f)) {
                         const float mn = fmaxf(m, mx);
                         const float alpha = m == -INFINITY ? 0.f : ex2_approx(m - mn);
@@ -468,67 +434,60 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                             }
                             tc_fence_after();
 #pragma unroll 1
-                            for (int c = 0; c < D / 64; ++c) {
-                                uint32_t o[32];
-                                tmem_ld32_wait(tO + c * 32, o);
+                            for (int c = 0; c < D / 16; ++c) {
+                                uint32_t o[16];
+                                tmem_ld16_wait(tO + c * 16, o);
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                                tmem_st32(tO + c * 32, o);
+                                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                                tmem_st16(tO + c * 16, o);
                             }
                         }
                     }
-                    // Pass 2: p = 2^(s - m); l sums the fp32 p; P, rounded to the inputs' type (half a step per key,
-                    // averaged over the row), goes into the columns already read: 32 scores -> 16 columns.
+                    // p = 2^(s - m); l sums the fp32 p; P, rounded to the inputs' type (half a step per key, averaged over
+                    // the row), goes over the scores already read: 32 scores -> 16 columns.
                     const uint64_t c2 = BIAS ? pk2(1.f, 1.f) : pk2(scale2, scale2);
                     const float nm = m == -INFINITY ? 0.f : -m;
                     const uint64_t nm2 = pk2(nm, nm);
-                    uint64_t l2 = pk2(0.f, 0.f);
+                    uint64_t l2 = pk2(0.f, 0.f), l3 = pk2(0.f, 0.f);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t v[32], pk[16];
-                        tmem_ld32_wait(tS + c * 32, v);
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t pk[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const int key = key0 + c * 32 + 2 * e;
-                            const float2 x = upk2(fma2(pk2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, nm2));
-                            float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
-                            if (!BIAS && !full) {
-                                if (key < lo || key >= hi) p0 = 0.f;
-                                if (key + 1 < lo || key + 1 >= hi) p1 = 0.f;
-                            }
-                            l2 = add2(l2, pk2(p0, p1));
+                            const int k = c * 32 + 2 * e;
+                            const float2 x = upk2(fma2(pk2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c2, nm2));
+                            const float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
+                            if (e & 1)
+                                l3 = add2(l3, pk2(p0, p1));
+                            else
+                                l2 = add2(l2, pk2(p0, p1));
                             pk[e] = Pair<T>::pack(p0, p1);
                         }
                         tmem_st16(tS + c * 16, pk);
+                        if (c == 1) {
+                            tmem_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&p_half[t]);
+                        }
                     }
-                    const float2 lf = upk2(l2);
+                    const float2 lf = upk2(add2(l2, l3));
                     l += lf.x + lf.y;
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&p_full[t]);
                 }
-                if (!ok) break;
-                // The row sum is the two halves' sums (half 0 first in both warps).
-                rl[hh] = l;
-                if (!pair_sync(pbar, pair_ph++ & 1, abort_flag)) {
-                    ok = false;
-                    break;
-                }
-                l = rl[0] + rl[1];
-                if (!mbar_wait(&o_done[t], (ucount - 1) & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE)) {
-                    ok = false;
-                    break;
-                }
+                if (!ok || !mbar_wait(&o_done[t], (ucount - 1) & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE)) break;
                 tc_fence_after();
                 const bool live = row < rows;
                 const int r = it.rt * ROWS + t * TQ + row;
                 const int tok = it.q0 + r / a.group, head = it.kvh * a.group + r % a.group;
                 if (it.slot < 0) {
                     const float inv = l == 0.f ? 0.f : 1.f / l;
-                    T* dst = static_cast<T*>(a.out) + (int64_t)tok * a.sot + (int64_t)head * a.soh + (D / 2) * hh;
+                    T* dst = static_cast<T*>(a.out) + (int64_t)tok * a.sot + (int64_t)head * a.soh;
 #pragma unroll 1
-                    for (int c = 0; c < D / 64; ++c) {
+                    for (int c = 0; c < D / 32; ++c) {
                         uint32_t o[32];
                         tmem_ld32_wait(tO + c * 32, o);
                         if (live) {
@@ -543,12 +502,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                             }
                         }
                     }
-                    if (a.lse && live && hh == 0) a.lse[(int64_t)tok * a.heads + head] = log_sum(m, l);
+                    if (a.lse && live) a.lse[(int64_t)tok * a.heads + head] = log_sum(m, l);
                 } else {
                     const int64_t srow = (int64_t)it.slot * ROWS + t * TQ + row;
-                    float* dst = a.part_o + srow * D + (D / 2) * hh;
+                    float* dst = a.part_o + srow * D;
 #pragma unroll 1
-                    for (int c = 0; c < D / 64; ++c) {
+                    for (int c = 0; c < D / 32; ++c) {
                         uint32_t o[32];
                         tmem_ld32_wait(tO + c * 32, o);
                         if (live) {
@@ -558,18 +517,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                                     make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                         }
                     }
-                    if (live && hh == 0) a.part_ml[srow] = make_float2(m, l);
+                    if (live) a.part_ml[srow] = make_float2(m, l);
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&o_free[t]);
             }
-            } while (next_list(count, false));
+        } while (next_list(count, false));
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == LOADERS) tmem_dealloc(tmem, 512);
+    if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
 template <class T, int D, bool BIAS>
