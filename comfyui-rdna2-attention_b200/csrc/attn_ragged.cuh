@@ -41,6 +41,7 @@ struct RaggedArgs {
     int batch, tokens, key_rows, heads, kv_heads, group;
     int causal, window;
     float scale, softcap;
+    int box_rows;  // rows of a TMA box (attn_tiles.cu)
     // workspace: partial O [slots][ROWS][D], (m, l) [slots][ROWS], item descriptor [CTAs][4]
     float* part_o;
     float2* part_ml;

@@ -110,15 +110,17 @@ __device__ __forceinline__ int fill_list(const RaggedArgs& a, Cursor* s_cur, Ite
     return cur.left > 0 ? n : -n;
 }
 
-template <class T, int D, bool BIAS>
-__global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_constant__ RaggedArgs a) {
+template <class T, int D, bool BIAS, bool TMA>
+__global__ void __launch_bounds__(THREADS, 1)
+    attn_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                      const __grid_constant__ RaggedArgs a) {
     using C = Cfg<D>;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t* q_full = bars + 0;   // 8 arrivals: row blocks of 32
     uint64_t* q_empty = bars + 1;
-    uint64_t* k_full = bars + 2;   // [2], 4 arrivals each
+    uint64_t* k_full = bars + 2;   // [2]: one TMA phase, or 4 arrivals (row blocks of 32)
     uint64_t* v_full = bars + 4;   // [2]
     uint64_t* k_empty = bars + 6;  // [2]
     uint64_t* v_empty = bars + 8;  // [2]
@@ -128,7 +130,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
     uint64_t* o_done = bars + 16;  // [2]
     uint64_t* o_free = bars + 18;  // [2]
     uint64_t* drain = bars + 20;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+    uint64_t* v_tail = bars + 21;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* list_len = abort_flag + 1;  // items in the list; negative: the last list
     Item* list = reinterpret_cast<Item*>(smem + C::OFF_LIST);
@@ -139,8 +142,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
         mbar_init(q_full, 8);
         mbar_init(q_empty, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], 4);
-            mbar_init(&v_full[i], 4);
+            mbar_init(&k_full[i], TMA ? 1 : 4);
+            mbar_init(&v_full[i], TMA ? 1 : 4);
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
@@ -150,6 +153,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
             mbar_init(&o_free[i], 4);
         }
         mbar_init(drain, 1);
+        mbar_init(v_tail, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -190,7 +194,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
         // Each role's code stands in the branch of its own register budget: behind a join the smaller one would hold.
         regs_dec<REGS_LOAD>();
         if (warp < 8 + LOADERS) {
-            const uint32_t loader = warp - 8;
+            // With TMA warp 8 loads keys and values and the other two the queries; else all three share all rows.
+            constexpr uint32_t Q_LOADERS = TMA ? LOADERS - 1 : LOADERS;
+            const uint32_t loader = warp - 8 - (TMA ? 1 : 0);
+            const bool tma_warp = TMA && warp == 8;
+            uint32_t tails = 0, k_issued = 0, v_issued = 0;
             uint32_t items_done = 0, units_done = 0, job = 0;
             int count;
             do {
@@ -222,44 +230,125 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                     s.len = it.len;
                     s.key0 = it.key0;
                     const int units = it.end - it.unit, first = it.unit, b = it.b;
-                    const T* kh = static_cast<const T*>(a.k) + it.kvh * a.s_head;
-                    const T* vh = static_cast<const T*>(a.v) + it.kvh * a.s_head;
-                    auto load_tile = [&](const T* base, unsigned char* ring, uint64_t* full, uint64_t* empty, int j) {
-                        const uint32_t u = units_done + j;
-                        const int st = u & 1;
+                    if (tma_warp) {
+                        // Lane -> box: `rows` keys of one page, 64 of their columns.
+                        const int rows = a.box_rows, boxes = UNIT / rows;
+                        const int bi = lane & (boxes - 1), half = lane / boxes;
+                        auto place = [&](int j) -> int2 {  // page and row in it of the lane's box of unit j
+                            const int key = (first + j) * UNIT + bi * rows;
+                            if (j >= units || key >= s.len) return make_int2(0, 0);
+                            if (!a.table) return make_int2(0, (int)s.key0 + key);
+                            const int pi = key / a.page_size;
+                            int page = a.table[(int64_t)b * a.table_ld + pi];
+                            if (page < 0 || page >= a.num_pages) {
+                                atomicOr(&g_status, B2_DEV_BAD_PAGE);
+                                page = a.num_pages;  // outside the map: zeros
+                            }
+                            return make_int2(page, key - pi * a.page_size);
+                        };
+                        // Boxes past the last key are not loaded; returns the number of the unit's keys that are there.
+                        auto load_unit = [&](const CUtensorMap* map, unsigned char* ring, uint64_t* full, uint64_t* empty,
+                                             int j, int2 at, uint64_t* bar) -> int {
+                            const uint32_t u = units_done + j;
+                            const int st = u & 1;
+                            const int keys = min(UNIT, s.len - (first + j) * UNIT);
+                            const int live = keys <= 0 ? 0 : (keys + rows - 1) / rows;
+                            if (!wait_free(&empty[st], ((u >> 1) & 1) ^ 1)) return -1;
+                            uint64_t* to = bar ? bar : &full[st];
+                            if (lane == 0) {
+                                if (live)
+                                    mbar_arrive_expect_tx(to, live * rows * (D * 2));
+                                else
+                                    mbar_arrive(to);
+                            }
+                            __syncwarp();
+                            if (half < D / 64 && bi < live)
+                                tma_load_4d(ring + st * C::TILE + half * (128 * 128) + bi * rows * 128, map, to, 64 * half, at.y,
+                                            it.kvh, at.x);
+                            return max(keys, 0);
+                        };
+                        int2 at = place(0);
+                        ok = load_unit(&tmK, sK, k_full, k_empty, 0, at, nullptr) >= 0;
+                        if (ok) ++k_issued;
+                        for (int j = 0; j < units && ok; ++j) {
+                            const int2 next = place(j + 1);
+                            if (j + 1 < units) {
+                                ok = load_unit(&tmK, sK, k_full, k_empty, j + 1, next, nullptr) >= 0;
+                                if (!ok) break;
+                                ++k_issued;
+                            }
+                            const bool tail = (first + j + 1) * UNIT > s.len;
+                            const int keys = load_unit(&tmV, sV, v_full, v_empty, j, at, tail ? v_tail : nullptr);
+                            ok = keys >= 0;
+                            if (ok && tail) {
+                                // Rows behind the last key hold whatever the page or the stage held before; the product
+                                // takes them times zero, so they must be finite.
+                                ok = mbar_wait(v_tail, tails & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_PRODUCER);
+                                if (!ok && !mbar_wait_drain(v_tail, tails & 1, 100000000ull))
+                                    atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
+                                ++tails;
+                                unsigned char* tile = sV + ((units_done + j) & 1) * C::TILE;
+                                for (int c = keys * 8 + lane; c < UNIT * 8; c += 32)
+#pragma unroll
+                                    for (int h = 0; h < D / 64; ++h)
+                                        *reinterpret_cast<uint4*>(tile + h * (128 * 128) + c * 16) = make_uint4(0, 0, 0, 0);
+                                fence_proxy_async_smem();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(&v_full[(units_done + j) & 1]);
+                            }
+                            if (ok) ++v_issued;
+                            at = next;
+                        }
+                    } else {
+                        const T* kh = static_cast<const T*>(a.k) + it.kvh * a.s_head;
+                        const T* vh = static_cast<const T*>(a.v) + it.kvh * a.s_head;
+                        auto load_unit = [&](const T* base, unsigned char* ring, uint64_t* full, uint64_t* empty, int j) {
+                            const uint32_t u = units_done + j;
+                            const int st = u & 1;
+                            bool waited = false;
+                            for (int blk = 0; blk < 4; ++blk) {
+                                if (job++ % Q_LOADERS != loader) continue;
+                                const int64_t off = key_row_offset(a, s, b, (first + j) * UNIT + 32 * blk + lane, &g_status);
+                                if (!waited && !wait_free(&empty[st], ((u >> 1) & 1) ^ 1)) return false;
+                                waited = true;
+                                copy_rows(ring + st * C::TILE, blk, base, off);
+                                pend.push(&full[st]);
+                            }
+                            return true;
+                        };
+                        if (!TMA) ok = load_unit(kh, sK, k_full, k_empty, 0);
                         bool waited = false;
-                        for (int blk = 0; blk < 4; ++blk) {
-                            if (job++ % LOADERS != loader) continue;
-                            const int64_t off = key_row_offset(a, s, b, (first + j) * UNIT + 32 * blk + lane, &g_status);
-                            if (!waited && !wait_free(&empty[st], ((u >> 1) & 1) ^ 1)) return false;
+                        for (int blk = 0; blk < 8 && ok; ++blk) {
+                            if (job++ % Q_LOADERS != loader) continue;
+                            if (!waited) ok = wait_free(q_empty, (items_done & 1) ^ 1);
                             waited = true;
-                            copy_rows(ring + st * C::TILE, blk, base, off);
-                            pend.push(&full[st]);
+                            if (!ok) break;
+                            // Query rows of the item: row r is token r / group, head r % group of the kv head's group.
+                            const int r = it.rt * ROWS + 32 * blk + lane;
+                            int64_t off = -1;
+                            if (r < it.n * a.group) {
+                                const int tok = r / a.group;
+                                off = (int64_t)(it.q0 + tok) * a.sqt + (int64_t)(it.kvh * a.group + r - tok * a.group) * a.sqh;
+                            }
+                            copy_rows(sQ + (blk >> 2) * C::TILE, blk & 3, static_cast<const T*>(a.q), off);
+                            pend.push(q_full);
                         }
-                        return true;
-                    };
-                    ok = load_tile(kh, sK, k_full, k_empty, 0);
-                    bool waited = false;
-                    for (int blk = 0; blk < 8 && ok; ++blk) {
-                        if (job++ % LOADERS != loader) continue;
-                        if (!waited) ok = wait_free(q_empty, (items_done & 1) ^ 1);
-                        waited = true;
-                        if (!ok) break;
-                        // Query rows of the item: row r is token r / group, head r % group of the kv head's group.
-                        const int r = it.rt * ROWS + 32 * blk + lane;
-                        int64_t off = -1;
-                        if (r < it.n * a.group) {
-                            const int tok = r / a.group;
-                            off = (int64_t)(it.q0 + tok) * a.sqt + (int64_t)(it.kvh * a.group + r - tok * a.group) * a.sqh;
+                        for (int j = 0; !TMA && j < units && ok; ++j) {
+                            if (j + 1 < units) ok = load_unit(kh, sK, k_full, k_empty, j + 1);
+                            if (ok) ok = load_unit(vh, sV, v_full, v_empty, j);
                         }
-                        copy_rows(sQ + (blk >> 2) * C::TILE, blk & 3, static_cast<const T*>(a.q), off);
-                        pend.push(q_full);
-                    }
-                    for (int j = 0; j < units && ok; ++j) {
-                        if (j + 1 < units) ok = load_tile(kh, sK, k_full, k_empty, j + 1);
-                        if (ok) ok = load_tile(vh, sV, v_full, v_empty, j);
+                        pend.drain(0);
                     }
                     units_done += units;
+                }
+                if (tma_warp && !ok) {
+                    // Given up: the copies in flight must land before the CTA ends.
+                    for (uint32_t n = 1; n <= 2; ++n) {
+                        if (k_issued >= n && !mbar_wait_drain(&k_full[(k_issued - n) & 1], ((k_issued - n) >> 1) & 1, 100000000ull))
+                            atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
+                        if (v_issued >= n && !mbar_wait_drain(&v_full[(v_issued - n) & 1], ((v_issued - n) >> 1) & 1, 100000000ull))
+                            atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
+                    }
                 }
                 pend.drain(0);
             } while (next_list(count, true));
@@ -531,11 +620,28 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
     if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-template <class T, int D, bool BIAS>
-int launch_tiles(const RaggedArgs& a, cudaStream_t s) {
-    if (int rc = set_smem(attn_tiles_kernel<T, D, BIAS>, Cfg<D>::SMEM)) return rc;
+// Tensor map of the keys or values: [pages][heads][rows][D], or one page of all packed rows.
+bool key_map(CUtensorMap* map, const void* base, const RaggedArgs& a, int dim, bool bf16) {
+    const bool paged = a.table != nullptr;
+    const uint64_t dims[4] = {(uint64_t)dim, (uint64_t)(paged ? a.page_size : a.key_rows), (uint64_t)a.kv_heads,
+                              (uint64_t)(paged ? a.num_pages : 1)};
+    const int64_t step[3] = {a.s_row * 2, a.s_head * 2, a.s_page * 2};
+    uint64_t strides[3];
+    for (int i = 0; i < 3; ++i) {
+        if (dims[i + 1] == 0) return false;
+        strides[i] = dims[i + 1] == 1 ? (uint64_t)dim * 2 : (uint64_t)step[i];  // a single row's stride is never used
+        if (strides[i] == 0 || strides[i] >= (1ull << 40)) return false;
+    }
+    const uint32_t box[4] = {64, (uint32_t)a.box_rows, 1, 1};
+    return make_map_4d(map, base, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, dims, strides,
+                       box) == B2_OK;
+}
+
+template <class T, int D, bool BIAS, bool TMA>
+int launch_tiles(const CUtensorMap& tk, const CUtensorMap& tv, const RaggedArgs& a, cudaStream_t s) {
+    if (int rc = set_smem(attn_tiles_kernel<T, D, BIAS, TMA>, Cfg<D>::SMEM)) return rc;
     const int ctas = sm_count();
-    attn_tiles_kernel<T, D, BIAS><<<ctas, THREADS, Cfg<D>::SMEM, s>>>(a);
+    attn_tiles_kernel<T, D, BIAS, TMA><<<ctas, THREADS, Cfg<D>::SMEM, s>>>(tk, tv, a);
     if (int rc = check_launch("attn_tiles_kernel")) return rc;
     return launch_merge(merge_kernel<T, D, ROWS>, a, ctas, ROWS, s);
 }
@@ -547,12 +653,24 @@ int64_t tiles_workspace(int dim) { return ragged_workspace(sm_count(), ROWS, dim
 int attn_tiles(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t s) {
     const bool bias = a.softcap > 0.f || a.slopes;
     ragged_slots(a, workspace, sm_count(), ROWS, dim);
-#define B2_TILES(T, D) return bias ? launch_tiles<T, D, true>(a, s) : launch_tiles<T, D, false>(a, s)
+    // A TMA box is as many rows as divide both a page and a unit; below 8 rows it would cut the swizzle's pattern, and a
+    // stride the map cannot hold has none: those caches are gathered by cp.async.
+    a.box_rows = a.table ? a.page_size & -a.page_size : UNIT;
+    if (a.box_rows > UNIT) a.box_rows = UNIT;
+    CUtensorMap tk{}, tv{};
+    const bool tma = a.box_rows >= 8 && key_map(&tk, a.k, a, dim, bf16) && key_map(&tv, a.v, a, dim, bf16);
+#define B2_TILES(T, D)                                                                                              \
+    if (tma) return bias ? launch_tiles<T, D, true, true>(tk, tv, a, s) : launch_tiles<T, D, false, true>(tk, tv, a, s); \
+    return bias ? launch_tiles<T, D, true, false>(tk, tv, a, s) : launch_tiles<T, D, false, false>(tk, tv, a, s)
     if (dim == 128) {
-        if (bf16) B2_TILES(__nv_bfloat16, 128);
+        if (bf16) {
+            B2_TILES(__nv_bfloat16, 128);
+        }
         B2_TILES(__half, 128);
     }
-    if (bf16) B2_TILES(__nv_bfloat16, 64);
+    if (bf16) {
+        B2_TILES(__nv_bfloat16, 64);
+    }
     B2_TILES(__half, 64);
 #undef B2_TILES
 }
