@@ -41,7 +41,8 @@ struct RaggedArgs {
     int batch, tokens, key_rows, heads, kv_heads, group;
     int causal, window;
     float scale, softcap;
-    int box_rows;  // rows of a TMA box (attn_tiles.cu)
+    int box_rows;  // attn_tiles.cu: rows of a TMA box of keys
+    int q_tma;     // and whether the queries come by TMA
     // workspace: partial O [slots][ROWS][D], (m, l) [slots][ROWS], item descriptor [CTAs][4]
     float* part_o;
     float2* part_ml;

@@ -16,7 +16,8 @@ namespace {
 __device__ unsigned int g_status;
 
 constexpr int TQ = 128, ROWS = 2 * TQ, UNIT = 128;
-constexpr int LOADERS = 3, MMA_WARP = 11;      // warps 0..7 softmax, 8..10 load, 11 issues the products
+// Warps 0..3 and 4..7: softmax of query tiles A and B; 8..10: loads; 11: the products.
+constexpr int LOADERS = 3, MMA_WARP = 11;
 constexpr int THREADS = 384, LIST_WRITER = 8 * 32;
 constexpr int LIST = 48;                      // items described in shared memory at a time
 // Registers: 168 a thread at launch; the loading warpgroup keeps 80, the two softmax warpgroups take 208:
@@ -112,13 +113,13 @@ __device__ __forceinline__ int fill_list(const RaggedArgs& a, Cursor* s_cur, Ite
 
 template <class T, int D, bool BIAS, bool TMA>
 __global__ void __launch_bounds__(THREADS, 1)
-    attn_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                      const __grid_constant__ RaggedArgs a) {
+    attn_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ RaggedArgs a) {
     using C = Cfg<D>;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-    uint64_t* q_full = bars + 0;   // 8 arrivals: row blocks of 32
+    uint64_t* q_full = bars + 0;   // one TMA phase, or 8 arrivals (row blocks of 32)
     uint64_t* q_empty = bars + 1;
     uint64_t* k_full = bars + 2;   // [2]: one TMA phase, or 4 arrivals (row blocks of 32)
     uint64_t* v_full = bars + 4;   // [2]
@@ -139,8 +140,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 8);
+        mbar_init(q_full, a.q_tma ? 1 : 8);
         mbar_init(q_empty, 1);
+        mbar_init(drain, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], TMA ? 1 : 4);
             mbar_init(&v_full[i], TMA ? 1 : 4);
@@ -152,7 +154,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(&o_done[i], 1);
             mbar_init(&o_free[i], 4);
         }
-        mbar_init(drain, 1);
         mbar_init(v_tail, 1);
         *abort_flag = 0;
         fence_mbar_init();
@@ -194,11 +195,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         // Each role's code stands in the branch of its own register budget: behind a join the smaller one would hold.
         regs_dec<REGS_LOAD>();
         if (warp < 8 + LOADERS) {
-            // With TMA warp 8 loads keys and values and the other two the queries; else all three share all rows.
+            // With TMA warp 8 loads keys and values (and the queries, if a box can hold them); else all share all rows.
             constexpr uint32_t Q_LOADERS = TMA ? LOADERS - 1 : LOADERS;
             const uint32_t loader = warp - 8 - (TMA ? 1 : 0);
             const bool tma_warp = TMA && warp == 8;
-            uint32_t tails = 0, k_issued = 0, v_issued = 0;
+            uint32_t tails = 0, k_issued = 0, v_issued = 0, q_issued = 0;
             uint32_t items_done = 0, units_done = 0, job = 0;
             int count;
             do {
@@ -270,6 +271,21 @@ __global__ void __launch_bounds__(THREADS, 1)
                         int2 at = place(0);
                         ok = load_unit(&tmK, sK, k_full, k_empty, 0, at, nullptr) >= 0;
                         if (ok) ++k_issued;
+                        if (ok && a.q_tma) {
+                            // 128 rows are 128 / group tokens of group heads. A second tile without rows is not loaded.
+                            ok = wait_free(q_empty, (items_done & 1) ^ 1);
+                            const int tiles = it.n * a.group - it.rt * ROWS > TQ ? 2 : 1;
+                            if (ok) {
+                                if (lane == 0) mbar_arrive_expect_tx(q_full, tiles * C::TILE);
+                                __syncwarp();
+                                if (lane < tiles * (D / 64)) {
+                                    const int t = lane / (D / 64), h = lane % (D / 64);
+                                    tma_load_4d(sQ + t * C::TILE + h * (128 * 128), &tmQ, q_full, 64 * h, it.kvh * a.group,
+                                                it.q0 + (it.rt * ROWS + t * TQ) / a.group, 0);
+                                }
+                                ++q_issued;
+                            }
+                        }
                         for (int j = 0; j < units && ok; ++j) {
                             const int2 next = place(j + 1);
                             if (j + 1 < units) {
@@ -299,7 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                             if (ok) ++v_issued;
                             at = next;
                         }
-                    } else {
+                    } else if (!TMA || !a.q_tma) {
                         const T* kh = static_cast<const T*>(a.k) + it.kvh * a.s_head;
                         const T* vh = static_cast<const T*>(a.v) + it.kvh * a.s_head;
                         auto load_unit = [&](const T* base, unsigned char* ring, uint64_t* full, uint64_t* empty, int j) {
@@ -343,6 +359,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 if (tma_warp && !ok) {
                     // Given up: the copies in flight must land before the CTA ends.
+                    if (q_issued && !mbar_wait_drain(q_full, (q_issued - 1) & 1, 100000000ull))
+                        atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
                     for (uint32_t n = 1; n <= 2; ++n) {
                         if (k_issued >= n && !mbar_wait_drain(&k_full[(k_issued - n) & 1], ((k_issued - n) >> 1) & 1, 100000000ull))
                             atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
@@ -353,92 +371,103 @@ __global__ void __launch_bounds__(THREADS, 1)
                 pend.drain(0);
             } while (next_list(count, true));
         } else {
+            // The products. The whole warp runs this role in step (waits by all lanes, their results voted, list entries
+            // broadcast) and one elected lane issues, so that the descriptors stay in uniform registers: with a lone lane
+            // in a divergent branch an issue took 70 to 100 cycles against the product's 64.
+            constexpr uint32_t FMT = __is_same(T, __nv_bfloat16) ? 1 : 0;
+            constexpr uint32_t idesc_qk = idesc_make(1, FMT, 0, 0, TQ, UNIT);
+            constexpr uint32_t idesc_pv = idesc_make(1, FMT, 0, 1, TQ, D);
+            const bool leader = elect_one();
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint64_t q_desc = sdesc_sw128(smem_u32(sQ), 16, 1024), k_desc = sdesc_sw128(smem_u32(sK), 16, 1024);
+            const uint64_t v_desc = sdesc_sw128(smem_u32(sV), 128 * 128, 1024);
             uint32_t items_done = 0, units_done = 0;
-            uint32_t tile_items[2] = {0, 0}, tile_units[2] = {0, 0};  // of query tile A (every item), B (items of > 128 rows)
-            int count;
-            do {
-                count = *list_len;
-                const int items = abs(count);
-                if (lane == 0) {
-                    constexpr uint32_t FMT = __is_same(T, __nv_bfloat16) ? 1 : 0;
-                    constexpr uint32_t idesc_qk = idesc_make(1, FMT, 0, 0, TQ, UNIT);
-                    constexpr uint32_t idesc_pv = idesc_make(1, FMT, 0, 1, TQ, D);
-                    auto wait = [&](uint64_t* bar, uint32_t parity) {
-                        return mbar_wait(bar, parity, abort_flag, &g_status, B2_DEV_TIMEOUT_MMA);
-                    };
-                    auto issue_s = [&](int t, int st) {
-                        const uint32_t k_addr = smem_u32(sK + st * C::TILE), q_addr = smem_u32(sQ + t * C::TILE);
+            uint32_t items_a = 0, units_a = 0, items_b = 0, units_b = 0;  // of tile A (every item), B (more than 128 rows)
+            auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+                return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, &g_status, B2_DEV_TIMEOUT_MMA));
+            };
+            auto issue_s = [&](const int t, uint32_t st) {
+                if (leader) {
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk) {
-                            const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
-                            mma_f16_ss(tmem + t * UNIT, sdesc_sw128(q_addr + off, 16, 1024), sdesc_sw128(k_addr + off, 16, 1024),
-                                       idesc_qk, kk != 0);
-                        }
-                        tc_commit(&s_full[t]);
-                    };
-                    // O of tile t += P V for unit j of the item: the first 64 keys as soon as their P is there.
-                    auto issue_pv = [&](int t, int st, int j) {
-                        const uint32_t v_addr = smem_u32(sV + st * C::TILE);
-                        const uint32_t ph = (tile_units[t] + j) & 1;
-                        if (!wait(&p_half[t], ph)) return false;
-                        // O is free once the softmax warps have read the tile's previous item out of it
-                        if (j == 0 && !wait(&o_free[t], (tile_items[t] & 1) ^ 1)) return false;
-                        tc_fence_after();
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+                        mma_f16_ss(tm + t * UNIT, q_desc + (t * C::TILE >> 4) + off, k_desc + st * (C::TILE >> 4) + off, idesc_qk,
+                                   kk != 0);
+                    }
+                    tc_commit(&s_full[t]);
+                }
+            };
+            // O of tile t += P V for unit j of the item, the n-th of the tile: the first 64 keys as soon as their P is there.
+            auto issue_pv = [&](const int t, uint32_t st, int j, uint32_t n, uint32_t item) -> bool {
+                if (!wait(&p_half[t], n & 1)) return false;
+                // O is free once the softmax warps have read the tile's previous item out of it
+                if (j == 0 && !wait(&o_free[t], (item & 1) ^ 1)) return false;
+                tc_fence_after();
 #pragma unroll
-                        for (int kk = 0; kk < 8; ++kk) {
-                            if (kk == 4) {
-                                if (!wait(&p_full[t], ph)) return false;
-                                tc_fence_after();
-                            }
-                            mma_f16_ts(tmem + 256 + t * D, tmem + t * UNIT + 8 * kk, sdesc_sw128(v_addr + kk * 2048, 128 * 128, 1024),
-                                       idesc_pv, (j | kk) != 0);
-                        }
-                        tc_commit(&o_done[t]);
-                        return true;
-                    };
-                    bool ok = true;
-                    for (int i = 0; i < items && ok; ++i, ++items_done) {
-                        const Item& it = list[i];
-                        const int units = it.end - it.unit;
-                        const bool two = it.n * a.group - it.rt * ROWS > TQ;
-                        uint32_t u = units_done;
-                        ok = wait(q_full, items_done & 1) && wait(&k_full[u & 1], (u >> 1) & 1);
-                        if (!ok) break;
+                for (int h = 0; h < 2; ++h) {
+                    if (h == 1) {
+                        if (!wait(&p_full[t], n & 1)) return false;
                         tc_fence_after();
-                        issue_s(0, u & 1);
-                        if (two) issue_s(1, u & 1);
-                        tc_commit(&k_empty[u & 1]);
-                        if (units == 1) tc_commit(q_empty);
-                        for (int j = 0; j < units; ++j, ++u) {
-                            const int st = u & 1, nx = (u + 1) & 1;
-                            const bool more = j + 1 < units;
-                            ok = wait(&v_full[st], (u >> 1) & 1) && issue_pv(0, st, j);
-                            if (ok && more) {
-                                ok = wait(&k_full[nx], ((u + 1) >> 1) & 1);
-                                if (ok) {
-                                    tc_fence_after();
-                                    issue_s(0, nx);
-                                }
-                            }
-                            if (ok && two) ok = issue_pv(1, st, j);
-                            if (!ok) break;
-                            tc_commit(&v_empty[st]);
-                            if (more) {
-                                if (two) issue_s(1, nx);
-                                tc_commit(&k_empty[nx]);
-                                if (j + 2 == units) tc_commit(q_empty);
-                            }
-                        }
-                        units_done += units;
-                        for (int t = 0; t <= (two ? 1 : 0); ++t) {
-                            tile_units[t] += units;
-                            ++tile_items[t];
-                        }
+                    }
+                    if (leader) {
+#pragma unroll
+                        for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                            mma_f16_ts(tm + 256 + t * D, tm + t * UNIT + 8 * kk, v_desc + st * (C::TILE >> 4) + kk * (2048 >> 4),
+                                       idesc_pv, kk == 0 ? (uint32_t)(j != 0) : 1u);
+                        if (h == 1) tc_commit(&o_done[t]);
                     }
                 }
-                __syncwarp();
+                return true;
+            };
+            int count;
+            do {
+                count = __shfl_sync(0xffffffffu, *list_len, 0);
+                const int items = abs(count);
+                bool ok = true;
+                for (int i = 0; i < items && ok; ++i, ++items_done) {
+                    const Item& it = list[i];
+                    const int units = __shfl_sync(0xffffffffu, it.end - it.unit, 0);
+                    const bool two = __shfl_sync(0xffffffffu, it.n * a.group - it.rt * ROWS, 0) > TQ;
+                    uint32_t u = units_done;
+                    ok = wait(q_full, items_done & 1) && wait(&k_full[u & 1], (u >> 1) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_s(0, u & 1);
+                    if (two) issue_s(1, u & 1);
+                    if (leader) {
+                        tc_commit(&k_empty[u & 1]);
+                        if (units == 1) tc_commit(q_empty);
+                    }
+                    for (int j = 0; j < units; ++j, ++u) {
+                        const uint32_t st = u & 1, nx = st ^ 1;
+                        const bool more = j + 1 < units;
+                        ok = wait(&v_full[st], (u >> 1) & 1) && issue_pv(0, st, j, units_a + j, items_a);
+                        if (ok && more) {
+                            ok = wait(&k_full[nx], ((u + 1) >> 1) & 1);
+                            if (ok) {
+                                tc_fence_after();
+                                issue_s(0, nx);
+                            }
+                        }
+                        if (ok && two) ok = issue_pv(1, st, j, units_b + j, items_b);
+                        if (!ok) break;
+                        if (more && two) issue_s(1, nx);
+                        if (leader) {
+                            tc_commit(&v_empty[st]);
+                            if (more) tc_commit(&k_empty[nx]);
+                            if (j + 2 == units) tc_commit(q_empty);
+                        }
+                    }
+                    units_done += units;
+                    units_a += units;
+                    ++items_a;
+                    if (two) {
+                        units_b += units;
+                        ++items_b;
+                    }
+                }
             } while (next_list(count, false));
-            if (lane == 0) {
+            if (leader) {
                 tc_commit(drain);
                 if (!mbar_wait_drain(drain, 0, 100000000ull)) atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
             }
@@ -637,11 +666,24 @@ bool key_map(CUtensorMap* map, const void* base, const RaggedArgs& a, int dim, b
                        box) == B2_OK;
 }
 
+// Tensor map of the queries, [tokens][heads][D] in boxes of 128 / group tokens of group heads.
+bool query_map(CUtensorMap* map, const RaggedArgs& a, int dim, bool bf16) {
+    if (TQ % a.group) return false;
+    const uint64_t dims[4] = {(uint64_t)dim, (uint64_t)a.heads, (uint64_t)a.tokens, 1};
+    const uint64_t strides[3] = {a.heads == 1 ? (uint64_t)dim * 2 : (uint64_t)a.sqh * 2,
+                                 a.tokens == 1 ? (uint64_t)dim * 2 : (uint64_t)a.sqt * 2, (uint64_t)dim * 2};
+    for (int i = 0; i < 2; ++i)
+        if (strides[i] == 0 || strides[i] >= (1ull << 40)) return false;
+    const uint32_t box[4] = {64, (uint32_t)a.group, (uint32_t)(TQ / a.group), 1};
+    return make_map_4d(map, a.q, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, dims, strides,
+                       box) == B2_OK;
+}
+
 template <class T, int D, bool BIAS, bool TMA>
-int launch_tiles(const CUtensorMap& tk, const CUtensorMap& tv, const RaggedArgs& a, cudaStream_t s) {
+int launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const RaggedArgs& a, cudaStream_t s) {
     if (int rc = set_smem(attn_tiles_kernel<T, D, BIAS, TMA>, Cfg<D>::SMEM)) return rc;
     const int ctas = sm_count();
-    attn_tiles_kernel<T, D, BIAS, TMA><<<ctas, THREADS, Cfg<D>::SMEM, s>>>(tk, tv, a);
+    attn_tiles_kernel<T, D, BIAS, TMA><<<ctas, THREADS, Cfg<D>::SMEM, s>>>(tq, tk, tv, a);
     if (int rc = check_launch("attn_tiles_kernel")) return rc;
     return launch_merge(merge_kernel<T, D, ROWS>, a, ctas, ROWS, s);
 }
@@ -657,11 +699,12 @@ int attn_tiles(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t 
     // stride the map cannot hold has none: those caches are gathered by cp.async.
     a.box_rows = a.table ? a.page_size & -a.page_size : UNIT;
     if (a.box_rows > UNIT) a.box_rows = UNIT;
-    CUtensorMap tk{}, tv{};
+    CUtensorMap tq{}, tk{}, tv{};
     const bool tma = a.box_rows >= 8 && key_map(&tk, a.k, a, dim, bf16) && key_map(&tv, a.v, a, dim, bf16);
+    a.q_tma = tma && query_map(&tq, a, dim, bf16);
 #define B2_TILES(T, D)                                                                                              \
-    if (tma) return bias ? launch_tiles<T, D, true, true>(tk, tv, a, s) : launch_tiles<T, D, false, true>(tk, tv, a, s); \
-    return bias ? launch_tiles<T, D, true, false>(tk, tv, a, s) : launch_tiles<T, D, false, false>(tk, tv, a, s)
+    if (tma) return bias ? launch_tiles<T, D, true, true>(tq, tk, tv, a, s) : launch_tiles<T, D, false, true>(tq, tk, tv, a, s); \
+    return bias ? launch_tiles<T, D, true, false>(tq, tk, tv, a, s) : launch_tiles<T, D, false, false>(tq, tk, tv, a, s)
     if (dim == 128) {
         if (bf16) {
             B2_TILES(__nv_bfloat16, 128);
