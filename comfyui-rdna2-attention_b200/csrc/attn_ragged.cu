@@ -64,6 +64,8 @@ extern "C" int b2_attn_ragged(const b2_attn_ragged_args* p, void* stream) {
     a.group = p->heads / p->kv_heads;
     a.causal = p->causal != 0;
     a.window = p->window >= (1 << 30) ? 0 : p->window;  // no position reaches that far
+    a.by_group.set(a.group);
+    if (a.table) a.by_page.set(a.page_size);
     a.scale = p->scale;
     a.softcap = p->softcap;
     auto kernel = few_rows(p->heads, p->kv_heads, p->max_q) ? attn_rows : attn_tiles;

@@ -24,6 +24,19 @@ namespace b2 {
 
 constexpr float RAGGED_LOG2E = 1.4426950408889634f;
 
+// x / d for 0 <= x < 2^31 and a fixed d, as a product and a shift: with l = ceil(log2 d) and m = floor(2^(31 + l) / d) + 1,
+// x m / 2^(31 + l) exceeds x / d by less than 1 / d.
+struct Divisor {
+    uint32_t m, shift;
+    void set(uint32_t d) {
+        uint32_t l = 0;
+        while ((1ull << l) < d) ++l;
+        m = (uint32_t)((1ull << (31 + l)) / d) + 1;
+        shift = 31 + l;
+    }
+    __device__ __forceinline__ int of(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> shift); }
+};
+
 struct RaggedArgs {
     const void* q;
     int64_t sqt, sqh;
@@ -41,6 +54,7 @@ struct RaggedArgs {
     int batch, tokens, key_rows, heads, kv_heads, group;
     int causal, window;
     float scale, softcap;
+    Divisor by_group, by_page;
     int box_rows;  // attn_tiles.cu: rows of a TMA box of keys
     int q_tma;     // and whether the queries come by TMA
     // workspace: partial O [slots][ROWS][D], (m, l) [slots][ROWS], item descriptor [CTAs][4]
@@ -82,8 +96,8 @@ __device__ __forceinline__ int key_lo(const RaggedArgs& a, const Sequence& s, in
 // The units [u0, u1) of the keys that any row of row tile rt sees.
 template <int ROWS, int UNIT>
 __device__ __forceinline__ int2 item_units(const RaggedArgs& a, const Sequence& s, int rt) {
-    const int tok0 = rt * ROWS / a.group;
-    const int tok1 = min(s.n - 1, (rt * ROWS + ROWS - 1) / a.group);
+    const int tok0 = a.by_group.of(rt * ROWS);
+    const int tok1 = min(s.n - 1, a.by_group.of(rt * ROWS + ROWS - 1));
     const int hi = key_hi(a, s, tok1), lo = key_lo(a, s, tok0);
     if (hi <= lo) return make_int2(0, 1);
     return make_int2(lo / UNIT, (hi + UNIT - 1) / UNIT);
@@ -92,23 +106,43 @@ template <int ROWS>
 __device__ __forceinline__ int row_tiles(const RaggedArgs& a, const Sequence& s) {
     return (s.n * a.group + ROWS - 1) / ROWS;
 }
-// Units of one kv head of a sequence.
+// Units of one kv head of each lane's sequence. A lane adds up a sequence of one or two row tiles by itself; the longer
+// ones are taken one after another by the whole warp, a row tile per lane.
 template <int ROWS, int UNIT>
 __device__ __forceinline__ int64_t head_units(const RaggedArgs& a, const Sequence& s) {
-    int64_t c = 0;
+    const int lane = threadIdx.x & 31;
     const int tiles = row_tiles<ROWS>(a, s);
-    for (int rt = 0; rt < tiles; ++rt) {
-        const int2 u = item_units<ROWS, UNIT>(a, s, rt);
-        c += u.y - u.x;
+    int64_t c = 0;
+    if (tiles <= 2)
+        for (int rt = 0; rt < tiles; ++rt) {
+            const int2 u = item_units<ROWS, UNIT>(a, s, rt);
+            c += u.y - u.x;
+        }
+    for (unsigned todo = __ballot_sync(0xffffffffu, tiles > 2); todo; todo &= todo - 1) {
+        const int src = __ffs(todo) - 1;
+        Sequence o{};
+        o.n = __shfl_sync(0xffffffffu, s.n, src);
+        o.len = __shfl_sync(0xffffffffu, s.len, src);
+        o.pos0 = __shfl_sync(0xffffffffu, s.pos0, src);
+        o.prefix = __shfl_sync(0xffffffffu, s.prefix, src);
+        const int many = row_tiles<ROWS>(a, o);
+        int64_t sum = 0;
+        for (int rt = lane; rt < many; rt += 32) {
+            const int2 u = item_units<ROWS, UNIT>(a, o, rt);
+            sum += u.y - u.x;
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == src) c = sum;
     }
     return c;
 }
 
 // The runs: run x is [begin(x), begin(x + 1)) of all units.
 struct Runs {
-    int64_t total;
-    int count;
-    __device__ __forceinline__ int64_t begin(int x) const { return total / count * x + total % count * x / count; }
+    int64_t each;  // units of a run; the first `more` runs have one more
+    int more, count;
+    __device__ __forceinline__ int64_t begin(int x) const { return each * x + min(x, more); }
 };
 
 // A CTA's place in the work: item (b, kvh, rt) with units [u0, u1), the next one to do and how many are left in its run.
@@ -124,13 +158,13 @@ template <int ROWS, int UNIT, int THREADS>
 __device__ __forceinline__ Cursor find_run(const RaggedArgs& a, int64_t* smem) {
     constexpr int WARPS = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto units_of = [&](int b) -> int64_t {
-        return b < a.batch ? head_units<ROWS, UNIT>(a, load_sequence(a, b)) * a.kv_heads : 0;
+    auto units_of = [&](int b) -> int64_t {  // every lane of the warp calls it
+        return head_units<ROWS, UNIT>(a, b < a.batch ? load_sequence(a, b) : Sequence{}) * a.kv_heads;
     };
     // Total, and each thread's count for the first THREADS sequences.
     const int64_t first = units_of(tid);
     int64_t sum = first;
-    for (int b = tid + THREADS; b < a.batch; b += THREADS) sum += units_of(b);
+    for (int b = THREADS; b < a.batch; b += THREADS) sum += units_of(b + tid);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) smem[warp] = sum;
@@ -139,15 +173,21 @@ __device__ __forceinline__ Cursor find_run(const RaggedArgs& a, int64_t* smem) {
     int64_t total = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) total += smem[w];
-    // Fewer units than CTAs: one each, the other CTAs have none.
     Cursor c;
-    c.runs.total = total;
+    // Fewer units than CTAs: one each, the other CTAs have none.
     c.runs.count = (int)min((int64_t)gridDim.x, total);
     c.left = 0;
     c.b = c.kvh = c.rt = c.u0 = c.u1 = c.unit = 0;
     c.s = Sequence{};
     __syncthreads();
     if ((int)blockIdx.x >= c.runs.count) return c;
+    if (total < (1ll << 32)) {
+        c.runs.each = (uint32_t)total / (uint32_t)c.runs.count;
+        c.runs.more = (uint32_t)total % (uint32_t)c.runs.count;
+    } else {
+        c.runs.each = total / c.runs.count;
+        c.runs.more = (int)(total % c.runs.count);
+    }
     const int64_t begin = c.runs.begin(blockIdx.x);
     c.left = c.runs.begin(blockIdx.x + 1) - begin;
     // The sequence that holds unit `begin`: prefix sums over THREADS sequences at a time.
@@ -168,6 +208,7 @@ __device__ __forceinline__ Cursor find_run(const RaggedArgs& a, int64_t* smem) {
         if (mine > 0 && lo <= begin && begin < lo + mine) {
             smem[34] = base + tid;
             smem[35] = begin - lo;
+            smem[36] = mine;
         }
         for (int w = 0; w < WARPS; ++w) before += smem[w];
         __syncthreads();
@@ -181,18 +222,35 @@ __device__ __forceinline__ Cursor find_run(const RaggedArgs& a, int64_t* smem) {
         return c;
     }
     c.s = load_sequence(a, c.b);
-    const int64_t per_head = head_units<ROWS, UNIT>(a, c.s);
-    c.kvh = (int)(rem / per_head);
-    rem -= c.kvh * per_head;
-    for (c.rt = 0;; ++c.rt) {
-        const int2 u = item_units<ROWS, UNIT>(a, c.s, c.rt);
-        if (rem < u.y - u.x) {
-            c.u0 = u.x;
-            c.u1 = u.y;
-            c.unit = u.x + (int)rem;
+    const int64_t per_head = smem[36] < (1ll << 32) ? (uint32_t)smem[36] / (uint32_t)a.kv_heads : smem[36] / a.kv_heads;
+    while (rem >= per_head) {
+        rem -= per_head;
+        ++c.kvh;
+    }
+    // The row tile: a tile per lane, prefix sums.
+    for (int rt0 = 0;; rt0 += 32) {
+        const int rt = rt0 + lane;
+        const int2 u = rt < row_tiles<ROWS>(a, c.s) ? item_units<ROWS, UNIT>(a, c.s, rt) : make_int2(0, 0);
+        int inc = u.y - u.x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += up;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, inc > rem);
+        if (past) {
+            const int src = __ffs(past) - 1;
+            c.rt = rt0 + src;
+            c.u0 = __shfl_sync(0xffffffffu, u.x, src);
+            c.u1 = __shfl_sync(0xffffffffu, u.y, src);
+            c.unit = c.u0 + (int)rem - __shfl_sync(0xffffffffu, inc, src) + c.u1 - c.u0;
             break;
         }
-        rem -= u.y - u.x;
+        rem -= __shfl_sync(0xffffffffu, inc, 31);
+        if (rt0 + 32 >= row_tiles<ROWS>(a, c.s)) {  // not reached: rem < per_head
+            c.left = 0;
+            break;
+        }
     }
     return c;
 }
@@ -237,7 +295,7 @@ __device__ __forceinline__ int64_t key_row_offset(const RaggedArgs& a, const Seq
                                                   unsigned int* status) {
     if (key >= s.len) return -1;
     if (!a.table) return (s.key0 + key) * a.s_row;
-    const int pi = key / a.page_size;
+    const int pi = a.by_page.of(key);
     const int page = a.table[(int64_t)b * a.table_ld + pi];
     if (page < 0 || page >= a.num_pages) {
         atomicOr(status, B2_DEV_BAD_PAGE);
@@ -319,7 +377,7 @@ __global__ void __launch_bounds__(512) merge_kernel(const RaggedArgs a) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    const int tok = s.q0 + r / a.group, head = d.z * a.group + r % a.group;
+    const int t = a.by_group.of(r), tok = s.q0 + t, head = d.z * a.group + r - t * a.group;
     T* dst = static_cast<T*>(a.out) + (int64_t)tok * a.sot + (int64_t)head * a.soh + lane * C;
     uint32_t u[C / 2];
 #pragma unroll

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const 
             const int row = (lane >> 2) + 8 * h;
             const bool live = row < rows;
             const int r = c.rt * ROWS + (live ? row : 0);
-            const int tok = r / a.group, head = c.kvh * a.group + r % a.group;
+            const int tok = a.by_group.of(r), head = c.kvh * a.group + r - tok * a.group;
             pos[h] = s.pos0 + tok;
             lo[h] = live ? key_lo(a, s, tok) : 0;
             hi[h] = live ? key_hi(a, s, tok) : 0x7fffffff;
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const 
             if (whole) {
                 const float inv = L == 0.f ? 0.f : 1.f / L;
                 const int r = c.rt * ROWS + row;
-                const int tok = s.q0 + r / a.group, head = c.kvh * a.group + r % a.group;
+                const int t = a.by_group.of(r), tok = s.q0 + t, head = c.kvh * a.group + r - t * a.group;
                 *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (int64_t)tok * a.sot + (int64_t)head * a.soh + col) =
                     make_uint4(Pair<T>::pack(v[0] * inv, v[1] * inv), Pair<T>::pack(v[2] * inv, v[3] * inv),
                                Pair<T>::pack(v[4] * inv, v[5] * inv), Pair<T>::pack(v[6] * inv, v[7] * inv));

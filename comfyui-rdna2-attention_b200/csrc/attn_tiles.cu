@@ -47,6 +47,74 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
+__device__ __forceinline__ uint64_t get2(const uint32_t (&v)[128], int e) {
+    return pk2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+}
+__device__ __forceinline__ void put2(uint32_t (&v)[128], int e, uint64_t x) {
+    const float2 f = upk2(x);
+    v[e] = __float_as_uint(f.x);
+    v[e + 1] = __float_as_uint(f.y);
+}
+
+// 2^x of a pair, x below 2^6, on the special-function unit (16 a cycle and SM)...
+__device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
+    const float2 f = upk2(x);
+    return pk2(ex2_approx(f.x), ex2_approx(f.y));
+}
+// ... and on the FMA units: 2^x = 2^n 2^f, n the nearest integer (from the bits of x + 1.5 * 2^23), f in [-1/2, 1/2];
+// 2^f by a polynomial of degree 4 fitted to the smallest relative error, 2.6e-6. Below 2^-126 the result is 2^-126 (it is
+// added to sums of at least 1 and rounds to 0 in 16 bits); a NaN stays one or becomes a huge value.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+    float2 c = upk2(x);
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(c.x));  // -126
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(c.y));
+    x = pk2(c.x, c.y);
+    const uint64_t magic = splat2(12582912.f);
+    const uint64_t r = add2(x, magic);
+    const uint64_t f = sub2(x, sub2(r, magic));
+    uint64_t p = fma2(splat2(0.009570101276040077f), f, splat2(0.05591785907745361f));
+    p = fma2(p, f, splat2(0.240247443318367f));
+    p = fma2(p, f, splat2(0.6931217908859253f));
+    p = fma2(p, f, splat2(0.9999992847442627f));
+    const float2 rf = upk2(r), pf = upk2(p);
+    return pk2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(rf.x) << 23)),
+               __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(rf.y) << 23)));
+}
+// One pair in POLY_EVERY goes to the FMA units: the special-function unit alone needs 2048 cycles for the 256 x 128
+// exponentials of a unit, as long as the tensor core for its four products.
+constexpr int POLY_EVERY = 4;
+
+// v = cap log2(e) tanh(y), y = cap_y v. Where the warp's |y| stay below 1 (scores well inside the cap), tanh(y) = y P(y^2)
+// with P of degree 5 fitted to the smallest relative error (6e-7), on pairs; else by exponential and reciprocal.
+__device__ __forceinline__ void cap_scores(uint32_t (&v)[128], float scale2, float cap_y, float cap_in, float cap2) {
+    float am[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 128; e += 8)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            am[q] = max3(am[q], fabsf(__uint_as_float(v[e + 2 * q])), fabsf(__uint_as_float(v[e + 2 * q + 1])));
+    const float top = max3(am[0], am[1], fmaxf(am[2], am[3])) * cap_y;
+    if (__all_sync(0xffffffffu, top <= 1.f)) {
+        const uint64_t k2 = splat2(cap_y * cap_y);
+        const uint64_t c0 = splat2(0.9999994039535522f * scale2), c1 = splat2(-0.3332904279232025f * scale2), c2 = splat2(0.13281433284282684f * scale2),
+                       c3 = splat2(-0.051605671644210815f * scale2), c4 = splat2(0.016743114218115807f * scale2), c5 = splat2(-0.0030670601408928633f * scale2);
+#pragma unroll
+        for (int e = 0; e < 128; e += 2) {
+            const uint64_t x = get2(v, e);
+            const uint64_t u = mul2(mul2(x, k2), x);
+            uint64_t p = fma2(c5, u, c4);
+            p = fma2(p, u, c3);
+            p = fma2(p, u, c2);
+            p = fma2(p, u, c1);
+            p = fma2(p, u, c0);
+            put2(v, e, mul2(x, p));  // cap2 y = scale2 x
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 128; ++e) v[e] = __float_as_uint(capped(__uint_as_float(v[e]) * cap_in, cap2));
+    }
+}
+
 // A loading warp's copies in flight: up to three groups, each with the barrier it completes.
 struct Pending {
     uint64_t* bar[3];
@@ -111,7 +179,7 @@ __device__ __forceinline__ int fill_list(const RaggedArgs& a, Cursor* s_cur, Ite
     return cur.left > 0 ? n : -n;
 }
 
-template <class T, int D, bool BIAS, bool TMA>
+template <class T, int D, int MODE, bool TMA>
 __global__ void __launch_bounds__(THREADS, 1)
     attn_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ RaggedArgs a) {
@@ -239,7 +307,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                             const int key = (first + j) * UNIT + bi * rows;
                             if (j >= units || key >= s.len) return make_int2(0, 0);
                             if (!a.table) return make_int2(0, (int)s.key0 + key);
-                            const int pi = key / a.page_size;
+                            const int pi = a.by_page.of(key);
                             int page = a.table[(int64_t)b * a.table_ld + pi];
                             if (page < 0 || page >= a.num_pages) {
                                 atomicOr(&g_status, B2_DEV_BAD_PAGE);
@@ -281,7 +349,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 if (lane < tiles * (D / 64)) {
                                     const int t = lane / (D / 64), h = lane % (D / 64);
                                     tma_load_4d(sQ + t * C::TILE + h * (128 * 128), &tmQ, q_full, 64 * h, it.kvh * a.group,
-                                                it.q0 + (it.rt * ROWS + t * TQ) / a.group, 0);
+                                                it.q0 + a.by_group.of(it.rt * ROWS + t * TQ), 0);
                                 }
                                 ++q_issued;
                             }
@@ -343,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                             const int r = it.rt * ROWS + 32 * blk + lane;
                             int64_t off = -1;
                             if (r < it.n * a.group) {
-                                const int tok = r / a.group;
+                                const int tok = a.by_group.of(r);
                                 off = (int64_t)(it.q0 + tok) * a.sqt + (int64_t)(it.kvh * a.group + r - tok * a.group) * a.sqh;
                             }
                             copy_rows(sQ + (blk >> 2) * C::TILE, blk & 3, static_cast<const T*>(a.q), off);
@@ -475,12 +543,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     } else {
         regs_inc<REGS_SOFTMAX>();
+        constexpr bool CAP = MODE & 1, SLOPE = MODE & 2;
         // Softmax: warps 0..3 tile A, 4..7 tile B; thread -> query row (TMEM lane), its 128 scores of a unit in registers.
         const int t = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lane_base + t * UNIT, tO = tmem + lane_base + 256 + t * D;
         const float scale2 = a.scale * RAGGED_LOG2E;
-        const float cap2 = a.softcap * RAGGED_LOG2E, cap_in = a.softcap > 0.f ? 2.f * scale2 / a.softcap : 0.f;
+        const float cap2 = a.softcap * RAGGED_LOG2E, cap_in = CAP ? 2.f * scale2 / a.softcap : 0.f;
+        const float cap_y = CAP ? a.scale / a.softcap : 0.f;  // tanh's argument per unit of raw score
         uint32_t ucount = 0;
         int count;
         do {
@@ -495,13 +565,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                 float slope = 0.f;
                 if (row < rows) {
                     const int r = it.rt * ROWS + t * TQ + row;
-                    const int tok = r / a.group;
+                    const int tok = a.by_group.of(r);
                     pos = it.pos0 + tok;
                     hi = a.causal ? min(it.len, max(pos + 1, it.prefix)) : it.len;
                     lo = a.window ? max(0, pos - a.window + 1) : 0;
-                    if (BIAS && a.slopes) slope = a.slopes[it.kvh * a.group + r - tok * a.group] * RAGGED_LOG2E;
+                    if (SLOPE) slope = a.slopes[it.kvh * a.group + r - tok * a.group] * RAGGED_LOG2E;
                 }
                 const int lo_all = __reduce_max_sync(0xffffffffu, lo), hi_all = __reduce_min_sync(0xffffffffu, hi);
+                // Keys a row may see behind its own position (their distance changes sign): first such key of the warp.
+                const int ahead = SLOPE && (!a.causal || it.prefix > 0)
+                                      ? __reduce_min_sync(0xffffffffu, row < rows ? pos : 0x7fffffff)
+                                      : 0x7fffffff;
                 float m = -INFINITY, l = 0.f;
                 bool ok = true;
                 for (int j = 0; j < units; ++j, ++ucount) {
@@ -513,14 +587,21 @@ __global__ void __launch_bounds__(THREADS, 1)
                     uint32_t v[128];
                     tmem_ld128_wait(tS, v);
                     const int key0 = (first + j) * UNIT;
-                    if (BIAS) {
-                        // finished scores in the base-2 domain
+                    // Finished scores in the base-2 domain, except where the scale is all there is to do (MODE 0).
+                    if (CAP) cap_scores(v, scale2, cap_y, cap_in, cap2);
+                    if (SLOPE) {
+                        const float dist = (float)(pos - key0);  // of key 0
+                        const uint64_t sc = CAP ? pk2(1.f, 1.f) : pk2(scale2, scale2);
+                        if (key0 + UNIT - 1 <= ahead) {
+                            const uint64_t s2 = pk2(slope, slope), b2 = pk2(-slope * dist, -slope * dist);
 #pragma unroll
-                        for (int e = 0; e < 128; ++e) {
-                            const float raw = __uint_as_float(v[e]);
-                            float y = raw * scale2;
-                            if (a.softcap > 0.f) y = capped(raw * cap_in, cap2);
-                            v[e] = __float_as_uint(fmaf(-slope, (float)abs(pos - key0 - e), y));
+                            for (int e = 0; e < 128; e += 2)
+                                put2(v, e, fma2(get2(v, e), sc, fma2(s2, pk2((float)e, (float)(e + 1)), b2)));
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 128; ++e)
+                                v[e] = __float_as_uint(fmaf(-slope, fabsf(dist - (float)e),
+                                                            __uint_as_float(v[e]) * (CAP ? 1.f : scale2)));
                         }
                     }
                     if (key0 < lo_all || key0 + UNIT > hi_all) {
@@ -536,7 +617,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         for (int q = 0; q < 4; ++q)
                             mm[q] = max3(mm[q], __uint_as_float(v[e + 2 * q]), __uint_as_float(v[e + 2 * q + 1]));
                     float mx = max3(mm[0], mm[1], fmaxf(mm[2], mm[3]));
-                    if (!BIAS) mx *= scale2;  // scale2 > 0
+                    if (MODE == 0) mx *= scale2;  // scale2 > 0
                     // The maximum moves only when a row's grew by more than 2^8: p stays below 2^8 (inside fp16) and O is
                     // rescaled rarely.
                     if (__any_sync(0xffffffffu, mx > m + 8.f)) {
@@ -563,7 +644,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                     // p = 2^(s - m); l sums the fp32 p; P, rounded to the inputs' type (half a step per key, averaged over
                     // the row), goes over the scores already read: 32 scores -> 16 columns.
-                    const uint64_t c2 = BIAS ? pk2(1.f, 1.f) : pk2(scale2, scale2);
+                    const uint64_t c2 = MODE ? pk2(1.f, 1.f) : pk2(scale2, scale2);
                     const float nm = m == -INFINITY ? 0.f : -m;
                     const uint64_t nm2 = pk2(nm, nm);
                     uint64_t l2 = pk2(0.f, 0.f), l3 = pk2(0.f, 0.f);
@@ -572,14 +653,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                         uint32_t pk[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const int k = c * 32 + 2 * e;
-                            const float2 x = upk2(fma2(pk2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c2, nm2));
-                            const float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
+                            const uint64_t x2 = fma2(get2(v, c * 32 + 2 * e), c2, nm2);
+                            const uint64_t pp = e % POLY_EVERY == POLY_EVERY - 1 ? exp2_poly(x2) : exp2_mufu(x2);
                             if (e & 1)
-                                l3 = add2(l3, pk2(p0, p1));
+                                l3 = add2(l3, pp);
                             else
-                                l2 = add2(l2, pk2(p0, p1));
-                            pk[e] = Pair<T>::pack(p0, p1);
+                                l2 = add2(l2, pp);
+                            const float2 p = upk2(pp);
+                            pk[e] = Pair<T>::pack(p.x, p.y);
                         }
                         tmem_st16(tS + c * 16, pk);
                         if (c == 1) {
@@ -600,7 +681,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tc_fence_after();
                 const bool live = row < rows;
                 const int r = it.rt * ROWS + t * TQ + row;
-                const int tok = it.q0 + r / a.group, head = it.kvh * a.group + r % a.group;
+                const int tr = a.by_group.of(r), tok = it.q0 + tr, head = it.kvh * a.group + r - tr * a.group;
                 if (it.slot < 0) {
                     const float inv = l == 0.f ? 0.f : 1.f / l;
                     T* dst = static_cast<T*>(a.out) + (int64_t)tok * a.sot + (int64_t)head * a.soh;
@@ -679,11 +760,11 @@ bool query_map(CUtensorMap* map, const RaggedArgs& a, int dim, bool bf16) {
                        box) == B2_OK;
 }
 
-template <class T, int D, bool BIAS, bool TMA>
+template <class T, int D, int MODE, bool TMA>
 int launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const RaggedArgs& a, cudaStream_t s) {
-    if (int rc = set_smem(attn_tiles_kernel<T, D, BIAS, TMA>, Cfg<D>::SMEM)) return rc;
+    if (int rc = set_smem(attn_tiles_kernel<T, D, MODE, TMA>, Cfg<D>::SMEM)) return rc;
     const int ctas = sm_count();
-    attn_tiles_kernel<T, D, BIAS, TMA><<<ctas, THREADS, Cfg<D>::SMEM, s>>>(tq, tk, tv, a);
+    attn_tiles_kernel<T, D, MODE, TMA><<<ctas, THREADS, Cfg<D>::SMEM, s>>>(tq, tk, tv, a);
     if (int rc = check_launch("attn_tiles_kernel")) return rc;
     return launch_merge(merge_kernel<T, D, ROWS>, a, ctas, ROWS, s);
 }
@@ -693,7 +774,7 @@ int launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap
 int64_t tiles_workspace(int dim) { return ragged_workspace(sm_count(), ROWS, dim); }
 
 int attn_tiles(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t s) {
-    const bool bias = a.softcap > 0.f || a.slopes;
+    const int mode = (a.softcap > 0.f ? 1 : 0) | (a.slopes ? 2 : 0);
     ragged_slots(a, workspace, sm_count(), ROWS, dim);
     // A TMA box is as many rows as divide both a page and a unit; below 8 rows it would cut the swizzle's pattern, and a
     // stride the map cannot hold has none: those caches are gathered by cp.async.
@@ -702,19 +783,23 @@ int attn_tiles(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t 
     CUtensorMap tq{}, tk{}, tv{};
     const bool tma = a.box_rows >= 8 && key_map(&tk, a.k, a, dim, bf16) && key_map(&tv, a.v, a, dim, bf16);
     a.q_tma = tma && query_map(&tq, a, dim, bf16);
-#define B2_TILES(T, D)                                                                                              \
-    if (tma) return bias ? launch_tiles<T, D, true, true>(tq, tk, tv, a, s) : launch_tiles<T, D, false, true>(tq, tk, tv, a, s); \
-    return bias ? launch_tiles<T, D, true, false>(tq, tk, tv, a, s) : launch_tiles<T, D, false, false>(tq, tk, tv, a, s)
+#define B2_TILES(T, D)                                                                                             \
+    switch (mode) {                                                                                                \
+        case 0: return tma ? launch_tiles<T, D, 0, true>(tq, tk, tv, a, s) : launch_tiles<T, D, 0, false>(tq, tk, tv, a, s); \
+        case 1: return tma ? launch_tiles<T, D, 1, true>(tq, tk, tv, a, s) : launch_tiles<T, D, 1, false>(tq, tk, tv, a, s); \
+        case 2: return tma ? launch_tiles<T, D, 2, true>(tq, tk, tv, a, s) : launch_tiles<T, D, 2, false>(tq, tk, tv, a, s); \
+        default: return tma ? launch_tiles<T, D, 3, true>(tq, tk, tv, a, s) : launch_tiles<T, D, 3, false>(tq, tk, tv, a, s); \
+    }
     if (dim == 128) {
         if (bf16) {
-            B2_TILES(__nv_bfloat16, 128);
+            B2_TILES(__nv_bfloat16, 128)
         }
-        B2_TILES(__half, 128);
+        B2_TILES(__half, 128)
     }
     if (bf16) {
-        B2_TILES(__nv_bfloat16, 64);
+        B2_TILES(__nv_bfloat16, 64)
     }
-    B2_TILES(__half, 64);
+    B2_TILES(__half, 64)
 #undef B2_TILES
 }
 
