@@ -63,15 +63,6 @@ SIGNATURES = {
 }
 
 
-class RaggedArgs(ctypes.Structure):
-    """b2_attn_ragged_args."""
-    _fields_ = ([("q", P), ("sqt", I64), ("sqh", I64), ("out", P), ("sot", I64), ("soh", I64), ("lse", P), ("k", P),
-                 ("v", P), ("s_page", I64), ("s_row", I64), ("s_head", I64), ("table", P), ("cu_q", P), ("lengths", P),
-                 ("prefix", P), ("slopes", P), ("workspace", P)]
-                + [(n, I) for n in ("table_ld", "max_pages", "num_pages", "page_size", "batch", "tokens", "key_rows",
-                                    "heads", "kv_heads", "dim", "dtype", "max_q", "causal", "window")]
-                + [("scale", F), ("softcap", F)])
-
 _lib = None
 
 

@@ -312,7 +312,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const 
 
 template <class T, int D, bool BIAS>
 int launch_rows(const RaggedArgs& a, cudaStream_t s) {
-    if (int rc = set_smem(attn_rows_kernel<T, D, BIAS>, Cfg<D>::SMEM)) return rc;
+    static bool done[64] = {false};
+    if (int rc = set_smem_once(attn_rows_kernel<T, D, BIAS>, Cfg<D>::SMEM, done)) return rc;
     const int ctas = Cfg<D>::CTAS * sm_count();
     attn_rows_kernel<T, D, BIAS><<<ctas, THREADS, Cfg<D>::SMEM, s>>>(a);
     if (int rc = check_launch("attn_rows_kernel")) return rc;

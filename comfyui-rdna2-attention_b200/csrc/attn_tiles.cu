@@ -762,7 +762,8 @@ bool query_map(CUtensorMap* map, const RaggedArgs& a, int dim, bool bf16) {
 
 template <class T, int D, int MODE, bool TMA>
 int launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const RaggedArgs& a, cudaStream_t s) {
-    if (int rc = set_smem(attn_tiles_kernel<T, D, MODE, TMA>, Cfg<D>::SMEM)) return rc;
+    static bool done[64] = {false};
+    if (int rc = set_smem_once(attn_tiles_kernel<T, D, MODE, TMA>, Cfg<D>::SMEM, done)) return rc;
     const int ctas = sm_count();
     attn_tiles_kernel<T, D, MODE, TMA><<<ctas, THREADS, Cfg<D>::SMEM, s>>>(tq, tk, tv, a);
     if (int rc = check_launch("attn_tiles_kernel")) return rc;

@@ -49,6 +49,18 @@ inline int set_smem(K kernel, int bytes) {
     return B2_OK;
 }
 
+// The same, once per kernel and device (`done`: a static array of the caller's).
+template <class K>
+inline int set_smem_once(K kernel, int bytes, bool (&done)[64]) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return set_smem(kernel, bytes);
+    if (!done[dev]) {
+        if (int rc = set_smem(kernel, bytes)) return rc;
+        done[dev] = true;
+    }
+    return B2_OK;
+}
+
 // Per-translation-unit device status words, read and cleared by b2_device_status().
 unsigned int read_status_gemm();
 unsigned int read_status_attention();

@@ -8,6 +8,7 @@ CUDA-tensor check, so they hold (and are tested) without a GPU.
 """
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -590,27 +591,38 @@ MAX_ROPE_PAIRS = 512
 BAD_PAGE = 16  # bit of _lib.device_status(): a page outside the cache was skipped
 
 
-def _on(t, fn):
-    """fn() with t's device current (the launch then goes to torch's current stream of that device)."""
-    if t.device.index == torch.cuda.current_device():
-        return fn()
-    with torch.cuda.device(t.device):
-        return fn()
+def _launch(name, device, *args):
+    """call() with ``device`` (its index) current, on torch's current stream of it."""
+    if device == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(device))
 
 
 def _one_device(t, *others):
-    require_cuda(t, *others)
+    """The index of the one CUDA device that every tensor given is on."""
+    device = t.get_device()
     for o in others:
-        if o is not None and o.device != t.device:
+        if o is not None and o.get_device() != device:
+            require_cuda(t, o)
             _fail(f"tensors on {t.device} and {o.device}: one call takes one device")
+    if device < 0:
+        require_cuda(t)
+    return device
 
 
-def _packed(t, name, like=None, dtypes=(torch.float16, torch.bfloat16, torch.float32)):
-    """[tokens, heads, dim] with a contiguous last dimension; ``like`` gives the dtype."""
-    if t.dim() != 3 or t.stride(2) != 1:
+def _packed(t, name, dtype=None):
+    """t as [tokens, heads, dim] with a contiguous last dimension (and of the given dtype): its shape and strides."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or (stride[2] != 1 and shape[2] != 1):
         _fail(f"{name} must be [tokens, heads, dim] with a contiguous last dimension")
-    if t.dtype not in dtypes or (like is not None and t.dtype != like.dtype):
-        _fail(f"{name} has dtype {t.dtype}, needs {like.dtype if like is not None else ' or '.join(map(str, dtypes))}")
+    if dtype is not None:
+        if t.dtype != dtype:
+            _fail(f"{name} has dtype {t.dtype}, needs {dtype}")
+    elif t.dtype not in _DTYPE_CODES:
+        _fail(f"{name} must be fp16, bf16 or fp32 (got {t.dtype})")
+    return shape, stride
 
 
 def _ints(t, n, name):
@@ -618,16 +630,21 @@ def _ints(t, n, name):
         _fail(f"{name} must be contiguous int32 [{n}] (got {t.dtype}, {tuple(t.shape)})")
 
 
-def _cache(k_cache, v_cache, table, kv_heads, dim, like, name):
-    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dim() != 4 or t.shape[2] != kv_heads or t.shape[3] != dim or t.stride(3) != 1 or t.dtype != like.dtype:
-            _fail(f"{name}: {n} must be {like.dtype} [pages, page_size, {kv_heads}, {dim}] with a contiguous last dimension")
-    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+def _cache(k_cache, v_cache, table, kv_heads, dim, dtype, name):
+    """The checks of a paged cache and its table; the cache's shape and strides and the table's."""
+    shape, stride = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or shape[2] != kv_heads or shape[3] != dim or (stride[3] != 1 and dim != 1):
+        _fail(f"{name}: k_cache must be [pages, page_size, {kv_heads}, {dim}] with a contiguous last dimension")
+    if v_cache.shape != shape or v_cache.stride() != stride:
         _fail(f"{name}: k_cache and v_cache must have equal shapes and strides")
-    if k_cache.shape[1] == 0:
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+        _fail(f"{name}: k_cache and v_cache must be {dtype} (got {k_cache.dtype}, {v_cache.dtype})")
+    if shape[1] == 0:
         _fail(f"{name}: pages of no rows")
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+    tshape, tstride = table.shape, table.stride()
+    if table.dtype != torch.int32 or len(tshape) != 2 or (tstride[1] != 1 and tshape[1] > 1):
         _fail(f"{name}: the page table must be int32 [batch, pages] with contiguous rows")
+    return shape, stride, tshape, tstride
 
 
 def rope_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_length=None, slow=1.0, fast=32.0, device=None):
@@ -685,19 +702,20 @@ def rope(x, positions, inv_freq, interleaved=False, mscale=1.0, out=None):
     turns by positions[t] * inv_freq[f]. Pairs are (f, f + len(inv_freq)), or (2f, 2f + 1) with ``interleaved``; values
     behind the 2 len(inv_freq) rotated ones are copied. Positions int64 [tokens]; negative ones turn back (the
     gradient of a rotation is the rotation by -positions). ``out`` may be x itself, but not overlap it otherwise."""
-    _packed(x, "rope x")
-    tokens, heads, dim = x.shape
+    shape, sx = _packed(x, "rope x")
+    tokens, heads, dim = shape
     pairs = _pairs(inv_freq, dim, "rope")
     _positions(positions, tokens, "rope")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        so = out.stride()
     else:
-        _packed(out, "rope output", x)
-        if out.shape != x.shape:
-            _fail(f"rope output has shape {tuple(out.shape)}, x {tuple(x.shape)}")
-    _one_device(x, positions, inv_freq, out)
-    _on(x, lambda: call("b2_rope", ptr(x), x.stride(0), x.stride(1), ptr(out), out.stride(0), out.stride(1), ptr(positions),
-                        ptr(inv_freq), mscale, tokens, heads, dim, pairs, int(interleaved), _DTYPE_CODES[x.dtype], stream()))
+        oshape, so = _packed(out, "rope output", x.dtype)
+        if oshape != shape:
+            _fail(f"rope output has shape {tuple(oshape)}, x {tuple(shape)}")
+    device = _one_device(x, positions, inv_freq, out)
+    _launch("b2_rope", device, x.data_ptr(), sx[0], sx[1], out.data_ptr(), so[0], so[1], positions.data_ptr(),
+            inv_freq.data_ptr(), mscale, tokens, heads, dim, pairs, 1 if interleaved else 0, _DTYPE_CODES[x.dtype])
     return out
 
 
@@ -712,56 +730,62 @@ def kv_append(k, v, k_cache, v_cache, table, cu_q, lengths, inv_freq=None, q=Non
     [batch] counts the sequence's positions with the new tokens, which are the last ones. Angles use these positions, or
     ``positions`` int64 [tokens]. Rows behind the last sequence are neither read into the cache nor written in q_out. A
     page outside the cache or a position outside the table drops that row and sets a bit of _lib.device_status()."""
-    _packed(k, "kv_append k")
-    _packed(v, "kv_append v", k)
-    tokens, kv_heads, dim = k.shape
-    if v.shape != k.shape or kv_heads == 0:
-        _fail(f"kv_append k and v must have equal shapes [tokens, kv_heads, dim] (got {tuple(k.shape)}, {tuple(v.shape)})")
-    _cache(k_cache, v_cache, table, kv_heads, dim, k, "kv_append")
-    batch = table.shape[0]
+    shape, sk = _packed(k, "kv_append k")
+    dtype = k.dtype
+    vshape, sv = _packed(v, "kv_append v", dtype)
+    tokens, kv_heads, dim = shape
+    if vshape != shape or kv_heads == 0:
+        _fail(f"kv_append k and v must have equal shapes [tokens, kv_heads, dim] (got {tuple(shape)}, {tuple(vshape)})")
+    cshape, sc, tshape, st = _cache(k_cache, v_cache, table, kv_heads, dim, dtype, "kv_append")
+    batch = tshape[0]
     _ints(cu_q, batch + 1, "kv_append cu_q")
     _ints(lengths, batch, "kv_append lengths")
     pairs = _pairs(inv_freq, dim, "kv_append")
     if positions is not None:
         _positions(positions, tokens, "kv_append")
-    heads = 0
+    heads, sq, so = 0, (0, 0), (0, 0)
     if q is not None:
-        _packed(q, "kv_append q", k)
-        if q.shape[0] != tokens or q.shape[2] != dim:
-            _fail(f"kv_append q must be [{tokens}, heads, {dim}] (got {tuple(q.shape)})")
-        heads = q.shape[1]
+        qshape, sq = _packed(q, "kv_append q", dtype)
+        heads = qshape[1]
+        if qshape[0] != tokens or qshape[2] != dim:
+            _fail(f"kv_append q must be [{tokens}, heads, {dim}] (got {tuple(qshape)})")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            so = q_out.stride()
         else:
-            _packed(q_out, "kv_append q_out", k)
-            if q_out.shape != q.shape:
-                _fail(f"kv_append q_out has shape {tuple(q_out.shape)}, q {tuple(q.shape)}")
+            oshape, so = _packed(q_out, "kv_append q_out", dtype)
+            if oshape != qshape:
+                _fail(f"kv_append q_out has shape {tuple(oshape)}, q {tuple(qshape)}")
     elif q_out is not None:
         _fail("kv_append: q_out without q")
-    _one_device(k, v, k_cache, v_cache, table, cu_q, lengths, inv_freq, positions, q, q_out)
-    sq = q.stride() if heads else (0, 0)
-    so = q_out.stride() if heads else (0, 0)
-    sc = k_cache.stride()
-    _on(k, lambda: call("b2_kv_append", ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), ptr(k_cache),
-                        ptr(v_cache), sc[0], sc[1], sc[2], ptr(table), table.stride(0), table.shape[1], k_cache.shape[0],
-                        k_cache.shape[1], ptr(cu_q), ptr(lengths), batch, ptr(q), sq[0], sq[1], ptr(q_out), so[0], so[1],
-                        ptr(positions), ptr(inv_freq), mscale, tokens, heads, kv_heads, dim, pairs, int(interleaved),
-                        _DTYPE_CODES[k.dtype], stream()))
+    device = _one_device(k, v, k_cache, v_cache, table, cu_q, lengths, inv_freq, positions, q, q_out)
+    _launch("b2_kv_append", device, k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], k_cache.data_ptr(),
+            v_cache.data_ptr(), sc[0], sc[1], sc[2], table.data_ptr(), st[0], tshape[1], cshape[0], cshape[1],
+            cu_q.data_ptr(), lengths.data_ptr(), batch, q.data_ptr() if heads else None, sq[0], sq[1],
+            q_out.data_ptr() if heads else None, so[0], so[1], positions.data_ptr() if positions is not None else None,
+            inv_freq.data_ptr() if pairs else None, mscale, tokens, heads, kv_heads, dim, pairs, 1 if interleaved else 0,
+            _DTYPE_CODES[dtype])
     return q_out
 
 
-def _attn_ragged(q, k, v, table, cu_q, lengths, batch, scale, causal, softcap, window, slopes, prefix, max_q, out, lse,
-                 workspace, name):
-    """The checks and the launch that attn_paged and attn_packed share (k, v: caches, or packed rows without a table)."""
-    tokens, heads, dim = q.shape
-    kv_heads = k.shape[-2]
-    if dim not in (64, 128):
+_RAGGED = struct.Struct("=QqqQqqQQQqqqQQQQQQ14i2f")  # b2_attn_ragged_args
+
+
+def _attn_ragged(name, q, qshape, sq, k, v, sk, kv_heads, table, table_dims, cu_q, lengths, batch, scale, causal, softcap,
+                 window, slopes, prefix, max_q, out, lse, workspace):
+    """The checks and the launch that attn_paged and attn_packed share (k, v: caches with strides sk = (page, row,
+    head) and table_dims = (row stride, pages per sequence, pages, page size), or packed rows without a table)."""
+    tokens, heads, dim = qshape
+    dtype = q.dtype
+    if dtype != torch.float16 and dtype != torch.bfloat16:
+        _fail(f"{name}: q must be fp16 or bf16 (got {dtype})")
+    if dim != 64 and dim != 128:
         _fail(f"{name}: head dim {dim} (64 or 128)")
     if kv_heads == 0 or heads == 0 or heads % kv_heads:
         _fail(f"{name}: {heads} query heads do not group over {kv_heads} KV heads")
-    _ints(cu_q, batch + 1, f"{name} cu_q")
+    _ints(cu_q, batch + 1, name + " cu_q")
     if prefix is not None:
-        _ints(prefix, batch, f"{name} prefix")
+        _ints(prefix, batch, name + " prefix")
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.dim() != 1 or slopes.shape[0] != heads
                                or not slopes.is_contiguous()):
         _fail(f"{name} slopes must be contiguous fp32 [{heads}]")
@@ -769,38 +793,39 @@ def _attn_ragged(q, k, v, table, cu_q, lengths, batch, scale, causal, softcap, w
     if not 0 < scale < 3e38 or not 0 <= softcap < 3e38 or window < 0:
         _fail(f"{name}: scale {scale} must be positive, softcap {softcap} and window {window} not negative")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        so = out.stride()
     else:
-        _packed(out, f"{name} output", q)
-        if out.shape != q.shape:
-            _fail(f"{name} output has shape {tuple(out.shape)}, q {tuple(q.shape)}")
+        oshape, so = _packed(out, name + " output", dtype)
+        if oshape != qshape:
+            _fail(f"{name} output has shape {tuple(oshape)}, q {tuple(qshape)}")
     if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (tokens, heads) or not lse.is_contiguous()):
         _fail(f"{name} lse must be contiguous fp32 [{tokens}, {heads}]")
-    if max_q is None:
-        max_q = -(-tokens // max(batch, 1))
-    _one_device(q, k, v, table, cu_q, lengths, prefix, slopes, out, lse, workspace)
-
-    def launch():
-        nbytes = _lib.load().b2_attn_ragged_workspace_bytes(heads, kv_heads, dim, max_q)
-        ws = workspace
-        if ws is None:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        elif not ws.is_contiguous() or ws.numel() * ws.element_size() < nbytes:
-            _fail(f"{name} workspace must be contiguous with at least {nbytes} bytes")
-        sq, so, sk = q.stride(), out.stride(), k.stride()
-        none = q.data_ptr()  # no keys at all: an empty tensor has no address, and nothing is read through this one
-        a = _lib.RaggedArgs(
-            q.data_ptr(), sq[0], sq[1], out.data_ptr(), so[0], so[1], 0 if lse is None else lse.data_ptr(),
-            k.data_ptr() or none, v.data_ptr() or none, 0 if table is None else sk[0], sk[-3], sk[-2], 0 if table is None else table.data_ptr(),
-            cu_q.data_ptr(), lengths.data_ptr(), 0 if prefix is None else prefix.data_ptr(),
-            0 if slopes is None else slopes.data_ptr(), ws.data_ptr(), 0 if table is None else table.stride(0),
-            0 if table is None else table.shape[1], k.shape[0], k.shape[1] if table is not None else 0, batch, tokens,
-            k.shape[0], heads, kv_heads, dim, _DTYPE_CODES[q.dtype], min(max_q, 1 << 30), int(causal), min(window, 1 << 30),
-            scale, softcap)
-        call("b2_attn_ragged", ctypes.byref(a), stream())
-
-    _on(q, launch)
+    max_q = -(-tokens // max(batch, 1)) if max_q is None else min(max(int(max_q), 0), 1 << 30)
+    device = _one_device(q, k, v, table, cu_q, lengths, prefix, slopes, out, lse, workspace)
+    if device == torch._C._cuda_getDevice():
+        nbytes = _ragged_workspace(heads, kv_heads, dim, max_q)
+    else:
+        with torch.cuda.device(device):
+            nbytes = _ragged_workspace(heads, kv_heads, dim, max_q)
+    if workspace is None:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < nbytes:
+        _fail(f"{name} workspace must be contiguous with at least {nbytes} bytes")
+    none = q.data_ptr()  # no keys at all: an empty tensor has no address, and nothing is read through this one
+    ld, max_pages, pages, page_size = table_dims
+    args = _RAGGED.pack(
+        none, sq[0], sq[1], out.data_ptr(), so[0], so[1], 0 if lse is None else lse.data_ptr(), k.data_ptr() or none,
+        v.data_ptr() or none, *sk, 0 if table is None else table.data_ptr() or none,
+        cu_q.data_ptr(), lengths.data_ptr(), 0 if prefix is None else prefix.data_ptr(),
+        0 if slopes is None else slopes.data_ptr(), workspace.data_ptr(), ld, max_pages, pages, page_size, batch, tokens,
+        k.shape[0], heads, kv_heads, dim, _DTYPE_CODES[dtype], max_q, 1 if causal else 0, min(window, 1 << 30), scale, softcap)
+    _launch("b2_attn_ragged", device, args)
     return out
+
+
+def _ragged_workspace(*args):
+    return _lib.load().b2_attn_ragged_workspace_bytes(*args)
 
 
 def attn_paged(q, k_cache, v_cache, table, cu_q, lengths, scale=None, causal=True, softcap=0.0, window=0, slopes=None,
@@ -815,13 +840,16 @@ def attn_paged(q, k_cache, v_cache, table, cu_q, lengths, scale=None, causal=Tru
     (fp32 [tokens, heads]) receives log sum exp(s). ``max_q``, the new tokens of the longest sequence, chooses the kernel
     (default: the mean). ``workspace`` (b2_attn_ragged_workspace_bytes, allocated when not given) must not be shared by
     calls that overlap on the GPU."""
-    _packed(q, "attn_paged q", None, (torch.float16, torch.bfloat16))
+    qshape, sq = _packed(q, "attn_paged q")
     if k_cache.dim() != 4:
         _fail("attn_paged: k_cache must be [pages, page_size, kv_heads, dim]")
-    _cache(k_cache, v_cache, table, k_cache.shape[2], q.shape[2], q, "attn_paged")
-    _ints(lengths, table.shape[0], "attn_paged lengths")
-    return _attn_ragged(q, k_cache, v_cache, table, cu_q, lengths, table.shape[0], scale, causal, softcap, window, slopes,
-                        prefix, max_q, out, lse, workspace, "attn_paged")
+    kv_heads = k_cache.shape[2]
+    cshape, sc, tshape, st = _cache(k_cache, v_cache, table, kv_heads, qshape[2], q.dtype, "attn_paged")
+    batch = tshape[0]
+    _ints(lengths, batch, "attn_paged lengths")
+    return _attn_ragged("attn_paged", q, qshape, sq, k_cache, v_cache, sc[:3], kv_heads, table,
+                        (st[0], tshape[1], cshape[0], cshape[1]), cu_q, lengths, batch, scale, causal, softcap, window, slopes,
+                        prefix, max_q, out, lse, workspace)
 
 
 def attn_packed(q, k, v, cu_q, cu_k, scale=None, causal=True, softcap=0.0, window=0, slopes=None, prefix=None, max_q=None,
@@ -829,16 +857,17 @@ def attn_packed(q, k, v, cu_q, cu_k, scale=None, causal=True, softcap=0.0, windo
     """attn_paged without a cache: sequence b's keys and values are rows cu_k[b] .. cu_k[b + 1] of k and v [keys, kv_heads,
     dim] (equal strides), so documents packed end to end each attend inside themselves. Where a sequence has more keys
     than queries, its queries are the last positions; the options are attn_paged's."""
-    _packed(q, "attn_packed q", None, (torch.float16, torch.bfloat16))
-    _packed(k, "attn_packed k", q)
-    _packed(v, "attn_packed v", q)
-    if k.shape != v.shape or k.stride() != v.stride() or k.shape[2] != q.shape[2]:
+    qshape, sq = _packed(q, "attn_packed q")
+    kshape, sk = _packed(k, "attn_packed k", q.dtype)
+    vshape, sv = _packed(v, "attn_packed v", q.dtype)
+    if vshape != kshape or sv != sk or kshape[2] != qshape[2]:
         _fail("attn_packed k and v must be [keys, kv_heads, dim] with q's dim and equal shapes and strides")
     if cu_q.dim() != 1 or cu_q.shape[0] < 1:
         _fail("attn_packed cu_q must be int32 [batch + 1]")
-    _ints(cu_k, cu_q.shape[0], "attn_packed cu_k")
-    return _attn_ragged(q, k, v, None, cu_q, cu_k, cu_q.shape[0] - 1, scale, causal, softcap, window, slopes, prefix, max_q,
-                        out, lse, workspace, "attn_packed")
+    batch = cu_q.shape[0] - 1
+    _ints(cu_k, batch + 1, "attn_packed cu_k")
+    return _attn_ragged("attn_packed", q, qshape, sq, k, v, (0, sk[0], sk[1]), kshape[1], None, (0, 0, 0, 0), cu_q, cu_k, batch, scale,
+                        causal, softcap, window, slopes, prefix, max_q, out, lse, workspace)
 
 
 def default_scale():

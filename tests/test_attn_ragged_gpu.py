@@ -8,6 +8,12 @@ from test_rope_gpu import paged
 pytestmark = pytest.mark.gpu
 
 F16, BF16 = torch.float16, torch.bfloat16
+# Rows per KV head (tokens x group) that max_q announces: one for each kernel.
+ROWS = [1, 1000]
+
+
+def hint(rows, group):
+    return -(-rows // group)
 
 
 def fill(kc, vc, table, lengths, seed):
@@ -72,11 +78,11 @@ def test_attn_paged(pkg, dev, dtype, batch, option):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("max_q", [1, 1000])
+@pytest.mark.parametrize("rows", ROWS)
 @pytest.mark.parametrize("nq,nk,H,Hk,D", [([5, 200, 1, 0, 33], [5, 200, 1, 0, 33], 4, 2, 128),
                                           ([1, 20, 129], [700, 20, 400], 5, 5, 64), ([4, 3], [0, 2], 8, 1, 128),
                                           ([2, 0], [0, 0], 2, 1, 64)])
-def test_attn_packed(pkg, dev, dtype, max_q, nq, nk, H, Hk, D):
+def test_attn_packed(pkg, dev, dtype, rows, nq, nk, H, Hk, D):
     """Documents in one buffer, more keys than queries, fewer keys than queries (positions below zero see nothing
     without a prefix), no keys at all."""
     starts = lambda c: torch.tensor([0] + list(torch.tensor(c).cumsum(0)), dtype=torch.int32, device=dev)
@@ -86,29 +92,29 @@ def test_attn_packed(pkg, dev, dtype, max_q, nq, nk, H, Hk, D):
     kv[sum(nk):] = float("nan")
     k, v = kv[:sum(nk), :Hk], kv[:sum(nk), Hk:]
     lse = torch.empty((sum(nq), H), device=dev)
-    out = pkg.ops.attn_packed(q, k, v, starts(nq), starts(nk), lse=lse, max_q=max_q)
+    out = pkg.ops.attn_packed(q, k, v, starts(nq), starts(nk), lse=lse, max_q=hint(rows, H // Hk))
     ends = torch.tensor(nk).cumsum(0).tolist()
     verify(out, lse, q, nq, lambda b: k[ends[b] - nk[b]:ends[b]], lambda b: v[ends[b] - nk[b]:ends[b]], {}, None, dtype, None)
 
 
-@pytest.mark.parametrize("max_q", [1, 64])
-def test_long_context_is_joined_from_parts(pkg, dev, max_q):
+@pytest.mark.parametrize("rows", ROWS)
+def test_long_context_is_joined_from_parts(pkg, dev, rows):
     """40000 keys for few rows: every item is cut over many CTAs; the same call twice gives the same bits."""
     counts, ctx = [1, 2, 1], [40000, 3, 9000]
     kc, vc, table, cu, lengths = paged(dev, F16, 2, 128, 16, counts, ctx, 5)
     fill(kc, vc, table, lengths, 5)
     q = (torch.randn((4, 8, 128), device=dev) * 3).half()
     lse = torch.empty((4, 8), device=dev)
-    out = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, lse=lse, max_q=max_q)
+    out = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, lse=lse, max_q=hint(rows, 4))
     total = lengths.tolist()
     verify(out, lse, q, counts, lambda b: pages_of(kc, table, b, total[b]), lambda b: pages_of(vc, table, b, total[b]),
            {}, None, F16, None)
-    assert torch.equal(out, pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, max_q=max_q))
+    assert torch.equal(out, pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, max_q=hint(rows, 4)))
 
 
-@pytest.mark.parametrize("max_q", [1, 64])
+@pytest.mark.parametrize("rows", ROWS)
 @pytest.mark.parametrize("B", [1, 700])
-def test_many_short_sequences(pkg, dev, B, max_q):
+def test_many_short_sequences(pkg, dev, B, rows):
     """More sequences than threads in a CTA, most of them shorter than a unit of keys, some without tokens."""
     counts = [(b * 7) % 3 for b in range(B - 1)] + [2]
     ctx = [(b * 13) % 90 for b in range(B)]
@@ -116,14 +122,14 @@ def test_many_short_sequences(pkg, dev, B, max_q):
     fill(kc, vc, table, lengths, 6)
     q = torch.randn((sum(counts), 4, 64), device=dev).to(BF16)
     lse = torch.empty((sum(counts), 4), device=dev)
-    out = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, lse=lse, max_q=max_q)
+    out = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, lse=lse, max_q=hint(rows, 4))
     total = lengths.tolist()
     verify(out, lse, q, counts, lambda b: pages_of(kc, table, b, total[b]), lambda b: pages_of(vc, table, b, total[b]),
            {}, None, BF16, None)
 
 
-@pytest.mark.parametrize("max_q", [1, 64])
-def test_extreme_scores(pkg, dev, max_q):
+@pytest.mark.parametrize("rows", ROWS)
+def test_extreme_scores(pkg, dev, rows):
     """Scores far apart (one key takes all), the types' lowest values among the keys, a cap that saturates."""
     n, m = 3, 200
     q = torch.zeros((n, 2, 64), device=dev).half()
@@ -135,34 +141,34 @@ def test_extreme_scores(pkg, dev, max_q):
     cu, ck = (torch.tensor([0, x], dtype=torch.int32, device=dev) for x in (n, m))
     for cap in (0.0, 3.0):
         lse = torch.empty((n, 2), device=dev)
-        out = pkg.ops.attn_packed(q, k, v, cu, ck, softcap=cap, lse=lse, max_q=max_q)
+        out = pkg.ops.attn_packed(q, k, v, cu, ck, softcap=cap, lse=lse, max_q=hint(rows, 2))
         want, l64, mass = attend64(q, k, v, softcap=cap)
         attend_check(out, want, mass, F16, m, v.abs().max().item())
         assert ((lse.double() - l64).abs() < 2e-4 + 1e-6 * l64.abs()).all()
 
 
-@pytest.mark.parametrize("max_q", [1, 64])
-def test_bad_pages_are_skipped(pkg, dev, max_q):
+@pytest.mark.parametrize("rows", ROWS)
+def test_bad_pages_are_skipped(pkg, dev, rows):
     kc, vc, table, cu, lengths = paged(dev, F16, 1, 64, 16, [2, 2], [60, 60], 8)
     fill(kc, vc, table, lengths, 8)
     q = torch.randn((4, 2, 64), device=dev).half()
-    good = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, max_q=max_q)
+    good = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, max_q=hint(rows, 2))
     assert pkg._lib.device_status() == 0
     for bad in (-5, kc.shape[0]):
         t2 = table.clone()
         t2[1, 1] = bad
-        out = pkg.ops.attn_paged(q, kc, vc, t2, cu, lengths, max_q=max_q)
+        out = pkg.ops.attn_paged(q, kc, vc, t2, cu, lengths, max_q=hint(rows, 2))
         assert pkg._lib.device_status() == pkg.ops.BAD_PAGE
         assert torch.equal(out[:2], good[:2]) and torch.isfinite(out).all()
     longer = torch.tensor([62, 1 << 30], dtype=torch.int32, device=dev)  # more keys than the table has rows for
     small = table[:, :4].contiguous()
-    out = pkg.ops.attn_paged(q, kc, vc, small, cu, longer, max_q=max_q)
+    out = pkg.ops.attn_paged(q, kc, vc, small, cu, longer, max_q=hint(rows, 2))
     assert torch.equal(out[:2], good[:2])
     pkg._lib.device_status()
 
 
-@pytest.mark.parametrize("max_q", [1, 64])
-def test_graph_replays_with_other_lengths(pkg, dev, max_q):
+@pytest.mark.parametrize("rows", ROWS)
+def test_graph_replays_with_other_lengths(pkg, dev, rows):
     """Append and attention captured once, replayed as the sequences grow, beside a second graph on another stream."""
     kc, vc, table, cu, lengths = paged(dev, BF16, 2, 128, 16, [1, 1, 1], [300, 20, 150], 9)
     fill(kc, vc, table, lengths, 9)
@@ -172,7 +178,7 @@ def test_graph_replays_with_other_lengths(pkg, dev, max_q):
 
     def step():
         qr = pkg.ops.kv_append(k, v, kc, vc, table, cu, lengths, inv_freq=inv, q=q)
-        return qr, pkg.ops.attn_paged(qr, kc, vc, table, cu, lengths, max_q=max_q)
+        return qr, pkg.ops.attn_paged(qr, kc, vc, table, cu, lengths, max_q=hint(rows, 2))
 
     step()
     graphs = []

@@ -12,10 +12,9 @@ H16 = torch.float16
 @pytest.fixture
 def calls(pkg, monkeypatch):
     log = []
-    monkeypatch.setattr(pkg.ops, "call", lambda name, *args: log.append((name, args)))
     monkeypatch.setattr(pkg.ops, "require_cuda", lambda *tensors: None)
-    monkeypatch.setattr(pkg.ops, "stream", lambda: None)
-    monkeypatch.setattr(pkg.ops, "_on", lambda t, fn: fn())
+    monkeypatch.setattr(pkg.ops, "_launch", lambda name, device, *args: log.append((name, args + (None,))))
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1, raising=False)  # a CPU tensor's device index
     return log
 
 
@@ -126,14 +125,13 @@ def test_cpu_tensors_are_refused(pkg):
 def test_c_entry_points_check_before_launching(pkg):
     lib, P = pkg._lib.load(), ctypes.c_void_p
     fake = P(4096)
-    good = dict(q=4096, sqt=512, sqh=64, out=4096, sot=512, soh=64, k=4096, v=4096, s_page=2048, s_row=128, s_head=64,
-                table=4096, cu_q=4096, lengths=4096, workspace=4096, table_ld=3, max_pages=3, num_pages=6, page_size=16,
+    good = dict(q=4096, sqt=512, sqh=64, out=4096, sot=512, soh=64, lse=0, k=4096, v=4096, s_page=2048, s_row=128, s_head=64,
+                table=4096, cu_q=4096, lengths=4096, prefix=0, slopes=0, workspace=4096, table_ld=3, max_pages=3, num_pages=6, page_size=16,
                 batch=2, tokens=5, key_rows=6, heads=8, kv_heads=2, dim=64, dtype=0, max_q=1, causal=1, window=0, scale=0.125,
                 softcap=0.0)
 
     def status(**kw):
-        a = pkg._lib.RaggedArgs(**{**good, **kw})
-        return lib.b2_attn_ragged(ctypes.byref(a), P(None))
+        return lib.b2_attn_ragged(pkg.ops._RAGGED.pack(*{**good, **kw}.values()), P(None))
 
     for kw in (dict(q=0), dict(out=0), dict(k=0), dict(cu_q=0), dict(lengths=0), dict(workspace=0), dict(heads=7),
                dict(kv_heads=0), dict(batch=-1), dict(window=-1), dict(scale=0.0), dict(scale=math.nan),
