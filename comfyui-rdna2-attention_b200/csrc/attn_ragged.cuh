@@ -358,12 +358,13 @@ __global__ void __launch_bounds__(512) merge_kernel(const RaggedArgs a) {
         if (p0 + lane < parts) {
             const float2 ml = a.part_ml[slot(p0 + lane)];
             w = ex2_approx(ml.x - ref);
-            L += w * ml.y;
+            if (w != 0.f) L += w * ml.y;
         }
         const int here = min(32, parts - p0);
 #pragma unroll 4
         for (int p = 0; p < here; ++p) {
             const float wp = __shfl_sync(0xffffffffu, w, p);
+            if (wp == 0.f) continue;  // a part that saw nothing may hold no O
             const float* src = a.part_o + slot(p0 + p) * D + lane * C;
             float v[C];
             if constexpr (C == 4)

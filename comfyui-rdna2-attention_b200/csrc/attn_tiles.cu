@@ -1,13 +1,19 @@
 // Ragged attention for many rows per kv head (chunks of prompts, packed documents): 256 rows per item on tcgen05.
 //
 // With 256 rows an item does 1024 D flops per key against 4 D bytes of keys and values, well above the 250 flops per
-// byte where the tensor cores become the bound. Each CTA works on two 128-row query tiles in ping-pong: while the
-// softmax warps of one tile work on its scores, the tensor core works on the other tile (S, P and O in TMEM, P written
-// back over the consumed scores as the A operand of the second product). One CTA per SM walks its run of units
-// (attn_ragged.cuh); every barrier's phase counts on across the items.
+// byte where the tensor cores become the bound. Two pipelines A and B work in ping-pong: while the softmax warps of one
+// work on its scores, the tensor core works for the other (S, P and O in TMEM, P written back over the consumed scores
+// as the A operand of the second product). An item of more than 128 rows puts its first 128 on A and the others on B,
+// each over the units that its own rows see. An item of up to 128 rows (short chunks, drafts being checked), which HBM
+// bounds, puts its even units on A and the odd ones on B, and the two results are joined at the end.
 //
-// Keys and values are gathered by rows (cp.async, 16 bytes a lane) into the 128-byte-swizzled layout that tcgen05 reads:
-// the page table's granularity is free, and rows behind the last key are zero-filled, so nothing stale is multiplied.
+// One CTA per SM walks its run of units (attn_ragged.cuh); every barrier's phase counts on across the items.
+//   warps 0..3, 4..7  softmax of A and B: thread -> row, its 128 scores of a unit in registers
+//   warp 8            TMA of keys and values (boxes of whole page parts) and queries
+//   warps 8..10       instead, the rows gathered by cp.async where no box fits (odd page sizes, odd groups for queries)
+//   warp 11           issues the products
+//   warps 12..15      epilogue: O out of TMEM while the softmax warps are at the next item
+// Rows behind a sequence's last key are zero in shared memory, so nothing stale is multiplied.
 #include "attn_ragged.cuh"
 
 namespace b2 {
@@ -16,16 +22,17 @@ namespace {
 __device__ unsigned int g_status;
 
 constexpr int TQ = 128, ROWS = 2 * TQ, UNIT = 128;
-// Warps 0..3 and 4..7: softmax of query tiles A and B; 8..10: loads; 11: the products.
-constexpr int LOADERS = 3, MMA_WARP = 11;
-constexpr int THREADS = 384, LIST_WRITER = 8 * 32;
-constexpr int LIST = 48;                      // items described in shared memory at a time
-// Registers: 168 a thread at launch; the loading warpgroup keeps 80, the two softmax warpgroups take 208:
-// 128 x 80 + 256 x 208 = 63488 of the launch's 384 x 168 = 64512.
-constexpr int REGS_LOAD = 80, REGS_SOFTMAX = 208;
+constexpr int LOADERS = 3, LOAD_WARP = 8, MMA_WARP = 11, EPI_WARP = 12;
+constexpr int THREADS = 512;
+constexpr int LIST = 48;  // items described in shared memory at a time
+// Registers: 128 a thread at launch; 128 x (2 x 176 (softmax) + 80 (loads, products) + 80 (epilogue)) = 512 x 128, the
+// split at which no role spills (200 / 56 / 56: packed documents 653 us against 577).
+constexpr int REGS_SOFTMAX = 176, REGS_LOAD = 80, REGS_EPI = 80;
 
 struct Item {
     int q0, n, len, pos0, prefix, b, kvh, rt, unit, end, slot;  // slot -1: the item is whole
+    int ub[2], ue[2];  // units of A and B, counted from `unit` (two tiles: every one; one tile: every second one)
+    int two;
     int64_t key0;
 };
 
@@ -35,7 +42,8 @@ struct Cfg {
     static constexpr int OFF_Q = 0;
     static constexpr int OFF_K = OFF_Q + 2 * TILE;
     static constexpr int OFF_V = OFF_K + 2 * TILE;
-    static constexpr int OFF_LIST = OFF_V + 2 * TILE;
+    static constexpr int OFF_ML = OFF_V + 2 * TILE;  // (m, l) of the rows of A and B
+    static constexpr int OFF_LIST = OFF_ML + 2 * TQ * 8;
     static constexpr int OFF_RUN = OFF_LIST + LIST * (int)sizeof(Item);
     static constexpr int OFF_CUR = OFF_RUN + 40 * 8;
     static constexpr int OFF_BAR = (OFF_CUR + (int)sizeof(Cursor) + 15) / 16 * 16;
@@ -47,72 +55,26 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
-__device__ __forceinline__ uint64_t get2(const uint32_t (&v)[128], int e) {
+template <int N>
+__device__ __forceinline__ uint64_t get2(const uint32_t (&v)[N], int e) {
     return pk2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
 }
-__device__ __forceinline__ void put2(uint32_t (&v)[128], int e, uint64_t x) {
+template <int N>
+__device__ __forceinline__ void put2(uint32_t (&v)[N], int e, uint64_t x) {
     const float2 f = upk2(x);
     v[e] = __float_as_uint(f.x);
     v[e + 1] = __float_as_uint(f.y);
 }
 
-// 2^x of a pair, x below 2^6, on the special-function unit (16 a cycle and SM)...
-__device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
-    const float2 f = upk2(x);
-    return pk2(ex2_approx(f.x), ex2_approx(f.y));
-}
-// ... and on the FMA units: 2^x = 2^n 2^f, n the nearest integer (from the bits of x + 1.5 * 2^23), f in [-1/2, 1/2];
-// 2^f by a polynomial of degree 4 fitted to the smallest relative error, 2.6e-6. Below 2^-126 the result is 2^-126 (it is
-// added to sums of at least 1 and rounds to 0 in 16 bits); a NaN stays one or becomes a huge value.
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
-    float2 c = upk2(x);
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(c.x));  // -126
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(c.y));
-    x = pk2(c.x, c.y);
-    const uint64_t magic = splat2(12582912.f);
-    const uint64_t r = add2(x, magic);
-    const uint64_t f = sub2(x, sub2(r, magic));
-    uint64_t p = fma2(splat2(0.009570101276040077f), f, splat2(0.05591785907745361f));
-    p = fma2(p, f, splat2(0.240247443318367f));
-    p = fma2(p, f, splat2(0.6931217908859253f));
-    p = fma2(p, f, splat2(0.9999992847442627f));
-    const float2 rf = upk2(r), pf = upk2(p);
-    return pk2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(rf.x) << 23)),
-               __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(rf.y) << 23)));
-}
-// One pair in POLY_EVERY goes to the FMA units: the special-function unit alone needs 2048 cycles for the 256 x 128
-// exponentials of a unit, as long as the tensor core for its four products.
-constexpr int POLY_EVERY = 4;
-
-// v = cap log2(e) tanh(y), y = cap_y v. Where the warp's |y| stay below 1 (scores well inside the cap), tanh(y) = y P(y^2)
-// with P of degree 5 fitted to the smallest relative error (6e-7), on pairs; else by exponential and reciprocal.
-__device__ __forceinline__ void cap_scores(uint32_t (&v)[128], float scale2, float cap_y, float cap_in, float cap2) {
-    float am[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < 128; e += 8)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            am[q] = max3(am[q], fabsf(__uint_as_float(v[e + 2 * q])), fabsf(__uint_as_float(v[e + 2 * q + 1])));
-    const float top = max3(am[0], am[1], fmaxf(am[2], am[3])) * cap_y;
-    if (__all_sync(0xffffffffu, top <= 1.f)) {
-        const uint64_t k2 = splat2(cap_y * cap_y);
-        const uint64_t c0 = splat2(0.9999994039535522f * scale2), c1 = splat2(-0.3332904279232025f * scale2), c2 = splat2(0.13281433284282684f * scale2),
-                       c3 = splat2(-0.051605671644210815f * scale2), c4 = splat2(0.016743114218115807f * scale2), c5 = splat2(-0.0030670601408928633f * scale2);
-#pragma unroll
-        for (int e = 0; e < 128; e += 2) {
-            const uint64_t x = get2(v, e);
-            const uint64_t u = mul2(mul2(x, k2), x);
-            uint64_t p = fma2(c5, u, c4);
-            p = fma2(p, u, c3);
-            p = fma2(p, u, c2);
-            p = fma2(p, u, c1);
-            p = fma2(p, u, c0);
-            put2(v, e, mul2(x, p));  // cap2 y = scale2 x
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 128; ++e) v[e] = __float_as_uint(capped(__uint_as_float(v[e]) * cap_in, cap2));
-    }
+// tanh(y) = y P(y^2), |y| <= 1, P of degree 5 fitted to the smallest relative error (7e-7): y P(y^2) scale on a pair.
+__device__ __forceinline__ uint64_t tanh_poly(uint64_t y, float scale) {
+    const uint64_t u = mul2(y, y);
+    uint64_t p = fma2(splat2(-0.0030670601408928633f * scale), u, splat2(0.016743114218115807f * scale));
+    p = fma2(p, u, splat2(-0.051605671644210815f * scale));
+    p = fma2(p, u, splat2(0.13281433284282684f * scale));
+    p = fma2(p, u, splat2(-0.3332904279232025f * scale));
+    p = fma2(p, u, splat2(0.9999994039535522f * scale));
+    return mul2(y, p);
 }
 
 // A loading warp's copies in flight: up to three groups, each with the barrier it completes.
@@ -152,31 +114,92 @@ struct Pending {
     }
 };
 
-// The CTA's next items into the list (one thread); returns their number, negative for the last list.
+// The CTA's next items into the list (one warp); returns their number, negative for the last list. An item of the
+// cursor's sequence per lane, cut where the run ends.
 __device__ __forceinline__ int fill_list(const RaggedArgs& a, Cursor* s_cur, Item* list) {
     Cursor cur = *s_cur;
+    const int lane = threadIdx.x & 31;
     int n = 0;
     while (cur.left > 0 && n < LIST) {
-        Item& it = list[n++];
-        const int end = (int)min((int64_t)cur.u1, cur.unit + cur.left);
-        it.q0 = cur.s.q0;
-        it.n = cur.s.n;
-        it.len = cur.s.len;
-        it.pos0 = cur.s.pos0;
-        it.prefix = cur.s.prefix;
-        it.key0 = cur.s.key0;
-        it.b = cur.b;
-        it.kvh = cur.kvh;
-        it.rt = cur.rt;
-        it.unit = cur.unit;
-        it.end = end;
-        it.slot = cur.unit == cur.u0 && end == cur.u1 ? -1 : 2 * (int)blockIdx.x + (cur.unit == cur.u0 ? 1 : 0);
-        if (cur.unit == cur.u0 && end < cur.u1)
-            a.desc[blockIdx.x] = make_int4(parts_after(cur, end), cur.b, cur.kvh, cur.rt);
-        advance<ROWS, UNIT>(a, cur, end - cur.unit);
+        const int tiles = row_tiles<ROWS>(a, cur.s);
+        const int f = cur.kvh * tiles + cur.rt + lane;  // items of the sequence: row tiles of kv head 0, of 1, ...
+        const int kvh = tiles == 1 ? f : f / tiles, rt = f - kvh * tiles;
+        const bool live = f < tiles * a.kv_heads;
+        const int2 u = live ? item_units<ROWS, UNIT>(a, cur.s, rt) : make_int2(0, 0);
+        const int start = lane == 0 ? cur.unit : u.x;
+        int inc = u.y - start;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += up;
+        }
+        const int64_t room = cur.left - (inc - (u.y - start));  // units of the run left for the lane's item
+        const bool take = live && room > 0 && n + lane < LIST;
+        const int end = (int)min((int64_t)u.y, start + room);
+        if (take) {
+            Item& it = list[n + lane];
+            it.q0 = cur.s.q0;
+            it.n = cur.s.n;
+            it.len = cur.s.len;
+            it.pos0 = cur.s.pos0;
+            it.prefix = cur.s.prefix;
+            it.key0 = cur.s.key0;
+            it.b = cur.b;
+            it.kvh = kvh;
+            it.rt = rt;
+            it.unit = start;
+            it.end = end;
+            it.slot = start == u.x && end == u.y ? -1 : 2 * (int)blockIdx.x + (start == u.x ? 1 : 0);
+            it.two = cur.s.n * a.group - rt * ROWS > TQ;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                int2 w = it.two ? item_units<TQ, UNIT>(a, cur.s, 2 * rt + t) : make_int2(start, end);
+                it.ub[t] = it.two ? min(max(w.x, start), end) - start : min(t, end - start);
+                it.ue[t] = max(min(w.y, end) - start, it.ub[t]);
+            }
+            if (start == u.x && end < u.y) {
+                cur.unit = start;  // for this lane's descriptor only
+                cur.u1 = u.y;
+                a.desc[blockIdx.x] = make_int4(parts_after(cur, end), cur.b, kvh, rt);
+            }
+        }
+        const int taken = __popc(__ballot_sync(0xffffffffu, take));
+        if (taken == 0) {  // not reached: units are left
+            cur.left = 0;
+            break;
+        }
+        const int used = __shfl_sync(0xffffffffu, inc, taken - 1);
+        cur.left = cur.left > used ? cur.left - used : 0;
+        n += taken;
+        // On to the item after the last one taken.
+        const int next = __shfl_sync(0xffffffffu, f, 0) + taken;
+        cur.kvh = next / tiles;
+        cur.rt = next - cur.kvh * tiles;
+        if (cur.left > 0) {
+            if (cur.kvh >= a.kv_heads) {
+                cur.kvh = cur.rt = 0;
+                do {
+                    if (++cur.b >= a.batch) {  // not reached: units are left
+                        cur.left = 0;
+                        break;
+                    }
+                    cur.s = load_sequence(a, cur.b);
+                } while (cur.s.n == 0);
+            }
+            if (cur.left > 0) cur.unit = item_units<ROWS, UNIT>(a, cur.s, cur.rt).x;
+        }
     }
-    *s_cur = cur;
+    __syncwarp();
+    if (lane == 0) *s_cur = cur;
     return cur.left > 0 ? n : -n;
+}
+
+// Which of 32 keys from key0 on a row sees, its keys being [lo, hi).
+__device__ __forceinline__ uint32_t seen_bits(int lo, int hi, int key0) {
+    const int l = lo - key0, h = hi - key0;
+    const uint32_t below = h >= 32 ? ~0u : h <= 0 ? 0u : (1u << h) - 1u;
+    const uint32_t from = l <= 0 ? ~0u : l >= 32 ? 0u : ~0u << l;
+    return below & from;
 }
 
 template <class T, int D, int MODE, bool TMA>
@@ -198,12 +221,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t* p_full = bars + 14;  // [2]
     uint64_t* o_done = bars + 16;  // [2]
     uint64_t* o_free = bars + 18;  // [2]
-    uint64_t* drain = bars + 20;
-    uint64_t* v_tail = bars + 21;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
+    uint64_t* ml_full = bars + 20; // [2]
+    uint64_t* drain = bars + 22;
+    uint64_t* v_tail = bars + 23;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* list_len = abort_flag + 1;  // items in the list; negative: the last list
     Item* list = reinterpret_cast<Item*>(smem + C::OFF_LIST);
+    float2* ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
 
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -220,7 +245,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(&p_half[i], 4);  // one arrival per softmax warp of the tile
             mbar_init(&p_full[i], 4);
             mbar_init(&o_done[i], 1);
-            mbar_init(&o_free[i], 4);
+            mbar_init(&o_free[i], 4);  // one per epilogue warp
+            mbar_init(&ml_full[i], 4);
         }
         mbar_init(v_tail, 1);
         *abort_flag = 0;
@@ -230,7 +256,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
-    // Thread 0 lists the CTA's next items; the cursor waits in shared memory meanwhile (it would cost every role's
+    // Warp LOAD_WARP lists the CTA's next items; the cursor waits in shared memory meanwhile (it would cost every role's
     // threads twenty registers).
     Cursor* s_cur = reinterpret_cast<Cursor*>(smem + C::OFF_CUR);
     {
@@ -240,7 +266,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
         }
     }
-    if (threadIdx.x == 0) *list_len = fill_list(a, s_cur, list);
+    __syncthreads();
+    if (warp == LOAD_WARP) {
+        const int n = fill_list(a, s_cur, list);
+        if (lane == 0) *list_len = n;
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -249,24 +279,27 @@ __global__ void __launch_bounds__(THREADS, 1)
     unsigned char* sK = smem + C::OFF_K;
     unsigned char* sV = smem + C::OFF_V;
 
-    // Every role walks the list, then meets the others where thread LIST_WRITER writes the next one (false: there is none,
-    // or a wait ran out). Phase counters run on across items and lists.
+    // Every role walks the list, then meets the others where warp LOAD_WARP writes the next one (false: there is none, or
+    // a wait ran out). Phase counters run on across items and lists.
     auto next_list = [&](int count, bool writer) -> bool {
         if (count <= 0) return false;
         __syncthreads();
-        if (writer && threadIdx.x == LIST_WRITER) *list_len = fill_list(a, s_cur, list);
+        if (writer && warp == LOAD_WARP) {
+            const int n = fill_list(a, s_cur, list);
+            if (lane == 0) *list_len = n;
+        }
         __syncthreads();
         return !*abort_flag;
     };
 
-    if (warp >= 8) {
-        // Each role's code stands in the branch of its own register budget: behind a join the smaller one would hold.
+    // Each role's code stands in the branch of its own register budget: behind a join the smaller one would hold.
+    if (warp >= LOAD_WARP && warp < EPI_WARP) {
         regs_dec<REGS_LOAD>();
-        if (warp < 8 + LOADERS) {
+        if (warp < LOAD_WARP + LOADERS) {
             // With TMA warp 8 loads keys and values (and the queries, if a box can hold them); else all share all rows.
             constexpr uint32_t Q_LOADERS = TMA ? LOADERS - 1 : LOADERS;
-            const uint32_t loader = warp - 8 - (TMA ? 1 : 0);
-            const bool tma_warp = TMA && warp == 8;
+            const uint32_t loader = warp - LOAD_WARP - (TMA ? 1 : 0);
+            const bool tma_warp = TMA && warp == LOAD_WARP;
             uint32_t tails = 0, k_issued = 0, v_issued = 0, q_issued = 0;
             uint32_t items_done = 0, units_done = 0, job = 0;
             int count;
@@ -342,7 +375,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         if (ok && a.q_tma) {
                             // 128 rows are 128 / group tokens of group heads. A second tile without rows is not loaded.
                             ok = wait_free(q_empty, (items_done & 1) ^ 1);
-                            const int tiles = it.n * a.group - it.rt * ROWS > TQ ? 2 : 1;
+                            const int tiles = it.two ? 2 : 1;
                             if (ok) {
                                 if (lane == 0) mbar_arrive_expect_tx(q_full, tiles * C::TILE);
                                 __syncwarp();
@@ -450,26 +483,26 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint64_t q_desc = sdesc_sw128(smem_u32(sQ), 16, 1024), k_desc = sdesc_sw128(smem_u32(sK), 16, 1024);
             const uint64_t v_desc = sdesc_sw128(smem_u32(sV), 128 * 128, 1024);
             uint32_t items_done = 0, units_done = 0;
-            uint32_t items_a = 0, units_a = 0, items_b = 0, units_b = 0;  // of tile A (every item), B (more than 128 rows)
+            uint32_t pv_a = 0, pv_b = 0, items_a = 0, items_b = 0;  // units and items that A and B have done
             auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
                 return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, &g_status, B2_DEV_TIMEOUT_MMA));
             };
-            auto issue_s = [&](const int t, uint32_t st) {
+            auto issue_s = [&](const int t, int q_tile, uint32_t st) {
                 if (leader) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
                         const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
-                        mma_f16_ss(tm + t * UNIT, q_desc + (t * C::TILE >> 4) + off, k_desc + st * (C::TILE >> 4) + off, idesc_qk,
-                                   kk != 0);
+                        mma_f16_ss(tm + t * UNIT, q_desc + q_tile * (C::TILE >> 4) + off, k_desc + st * (C::TILE >> 4) + off,
+                                   idesc_qk, kk != 0);
                     }
                     tc_commit(&s_full[t]);
                 }
             };
-            // O of tile t += P V for unit j of the item, the n-th of the tile: the first 64 keys as soon as their P is there.
-            auto issue_pv = [&](const int t, uint32_t st, int j, uint32_t n, uint32_t item) -> bool {
+            // O of pipeline t += P V, for its n-th unit: the first 64 keys as soon as their P is there. At an item's first
+            // unit O starts anew, once the epilogue has read the pipeline's previous item out of it.
+            auto issue_pv = [&](const int t, uint32_t st, bool first, uint32_t n, uint32_t item) -> bool {
                 if (!wait(&p_half[t], n & 1)) return false;
-                // O is free once the softmax warps have read the tile's previous item out of it
-                if (j == 0 && !wait(&o_free[t], (item & 1) ^ 1)) return false;
+                if (first && !wait(&o_free[t], (item & 1) ^ 1)) return false;
                 tc_fence_after();
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -481,7 +514,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                         for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
                             mma_f16_ts(tm + 256 + t * D, tm + t * UNIT + 8 * kk, v_desc + st * (C::TILE >> 4) + kk * (2048 >> 4),
-                                       idesc_pv, kk == 0 ? (uint32_t)(j != 0) : 1u);
+                                       idesc_pv, kk == 0 ? (first ? 0u : 1u) : 1u);
                         if (h == 1) tc_commit(&o_done[t]);
                     }
                 }
@@ -494,45 +527,75 @@ __global__ void __launch_bounds__(THREADS, 1)
                 bool ok = true;
                 for (int i = 0; i < items && ok; ++i, ++items_done) {
                     const Item& it = list[i];
-                    const int units = __shfl_sync(0xffffffffu, it.end - it.unit, 0);
-                    const bool two = __shfl_sync(0xffffffffu, it.n * a.group - it.rt * ROWS, 0) > TQ;
-                    uint32_t u = units_done;
-                    ok = wait(q_full, items_done & 1) && wait(&k_full[u & 1], (u >> 1) & 1);
+                    auto get = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+                    const int units = get(it.end - it.unit);
+                    const bool two = get(it.two);
+                    const int ab = get(it.ub[0]), ae = get(it.ue[0]), bb = get(it.ub[1]), be = get(it.ue[1]);
+                    const uint32_t u0 = units_done;
+                    auto stage = [&](int j) { return (u0 + j) & 1; };
+                    auto wait_k = [&](int j) {
+                        const bool there = wait(&k_full[stage(j)], ((u0 + j) >> 1) & 1);
+                        tc_fence_after();
+                        return there;
+                    };
+                    auto wait_v = [&](int j) { return wait(&v_full[stage(j)], ((u0 + j) >> 1) & 1); };
+                    ok = wait(q_full, items_done & 1) && wait_k(0);
                     if (!ok) break;
-                    tc_fence_after();
-                    issue_s(0, u & 1);
-                    if (two) issue_s(1, u & 1);
-                    if (leader) {
-                        tc_commit(&k_empty[u & 1]);
-                        if (units == 1) tc_commit(q_empty);
-                    }
-                    for (int j = 0; j < units; ++j, ++u) {
-                        const uint32_t st = u & 1, nx = st ^ 1;
-                        const bool more = j + 1 < units;
-                        ok = wait(&v_full[st], (u >> 1) & 1) && issue_pv(0, st, j, units_a + j, items_a);
-                        if (ok && more) {
-                            ok = wait(&k_full[nx], ((u + 1) >> 1) & 1);
-                            if (ok) {
-                                tc_fence_after();
-                                issue_s(0, nx);
+                    if (two) {
+                        if (ab == 0 && ae > 0) issue_s(0, 0, stage(0));
+                        if (bb == 0 && be > 0) issue_s(1, 1, stage(0));
+                        if (leader) {
+                            tc_commit(&k_empty[stage(0)]);
+                            if (units == 1) tc_commit(q_empty);
+                        }
+                        for (int j = 0; j < units; ++j) {
+                            const bool more = j + 1 < units;
+                            ok = wait_v(j);
+                            if (ok && ab <= j && j < ae) ok = issue_pv(0, stage(j), j == ab, pv_a++, items_a);
+                            if (ok && more) ok = wait_k(j + 1);
+                            if (!ok) break;
+                            if (ab <= j + 1 && j + 1 < ae) issue_s(0, 0, stage(j + 1));
+                            if (bb <= j && j < be) ok = issue_pv(1, stage(j), j == bb, pv_b++, items_b);
+                            if (!ok) break;
+                            if (bb <= j + 1 && j + 1 < be) issue_s(1, 1, stage(j + 1));
+                            if (leader) {
+                                tc_commit(&v_empty[stage(j)]);
+                                if (more) tc_commit(&k_empty[stage(j + 1)]);
+                                if (j + 2 == units) tc_commit(q_empty);
                             }
                         }
-                        if (ok && two) ok = issue_pv(1, st, j, units_b + j, items_b);
-                        if (!ok) break;
-                        if (more && two) issue_s(1, nx);
-                        if (leader) {
-                            tc_commit(&v_empty[st]);
-                            if (more) tc_commit(&k_empty[nx]);
-                            if (j + 2 == units) tc_commit(q_empty);
+                    } else {
+                        issue_s(0, 0, stage(0));
+                        if (leader) tc_commit(&k_empty[stage(0)]);
+                        if (units > 1) {
+                            ok = wait_k(1);
+                            if (!ok) break;
+                            issue_s(1, 0, stage(1));
+                            if (leader) tc_commit(&k_empty[stage(1)]);
+                        }
+                        if (leader && units <= 2) tc_commit(q_empty);
+                        // Unit j on pipeline j % 2, its next one after it.
+                        auto step = [&](const int t, int j, uint32_t n, uint32_t item) -> bool {
+                            if (!wait_v(j) || !issue_pv(t, stage(j), j == t, n, item)) return false;
+                            if (leader) tc_commit(&v_empty[stage(j)]);
+                            if (j + 2 < units) {
+                                if (!wait_k(j + 2)) return false;
+                                issue_s(t, 0, stage(j));
+                                if (leader) {
+                                    tc_commit(&k_empty[stage(j)]);
+                                    if (j + 3 == units) tc_commit(q_empty);
+                                }
+                            }
+                            return true;
+                        };
+                        for (int j = 0; j < units && ok; j += 2) {
+                            ok = step(0, j, pv_a++, items_a);
+                            if (ok && j + 1 < units) ok = step(1, j + 1, pv_b++, items_b);
                         }
                     }
                     units_done += units;
-                    units_a += units;
-                    ++items_a;
-                    if (two) {
-                        units_b += units;
-                        ++items_b;
-                    }
+                    items_a += ae > ab;
+                    items_b += be > bb;
                 }
             } while (next_list(count, false));
             if (leader) {
@@ -541,83 +604,238 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             __syncwarp();
         }
+    } else if (warp >= EPI_WARP) {
+        regs_dec<REGS_EPI>();
+        // Epilogue: rows out of TMEM, lane quarter warp % 4 of both pipelines.
+        const int row = (warp & 3) * 32 + lane;
+        const uint32_t tO = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256;
+        uint32_t done[2] = {0, 0}, units_of[2] = {0, 0};  // items and units of A and B
+        int count;
+        do {
+            count = *list_len;
+            const int items = abs(count);
+            bool ok = true;
+            for (int i = 0; i < items && ok; ++i) {
+                const Item& it = list[i];
+                const int two = it.two;
+                // m, l of pipeline t's part of the item; nothing seen where it has no units
+                auto arrive_at = [&](int t, int c, float2& w) -> bool {
+                    w = make_float2(-INFINITY, 0.f);
+                    if (c == 0) return true;
+                    units_of[t] += c;
+                    if (!mbar_wait(&ml_full[t], done[t] & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE) ||
+                        !mbar_wait(&o_done[t], (units_of[t] - 1) & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE))
+                        return false;
+                    w = ml[t * TQ + row];
+                    ++done[t];
+                    return true;
+                };
+                for (int p = 0; p <= two && ok; ++p) {  // two tiles: one after the other; one tile: both parts at once
+                    const int rows = it.n * a.group - it.rt * ROWS - p * TQ;
+                    const int ca = two ? it.ue[p] - it.ub[p] : (it.end - it.unit + 1) / 2;
+                    const int cb = two ? 0 : (it.end - it.unit) / 2;
+                    float2 wa, wb = make_float2(-INFINITY, 0.f);
+                    ok = arrive_at(p, ca, wa) && (two || arrive_at(1, cb, wb));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float M = fmaxf(wa.x, wb.x);
+                    float fa = wa.x == -INFINITY ? 0.f : ex2_approx(wa.x - M), fb = wb.x == -INFINITY ? 0.f : ex2_approx(wb.x - M);
+                    const float L = (ca ? wa.y * fa : 0.f) + (cb ? wb.y * fb : 0.f);
+                    const bool live = row < rows;
+                    const int r = it.rt * ROWS + p * TQ + row;
+                    const int tr = a.by_group.of(r), tok = it.q0 + tr, head = it.kvh * a.group + r - tr * a.group;
+                    const bool whole = it.slot < 0;
+                    const int64_t srow = (int64_t)it.slot * ROWS + p * TQ + row;
+                    if (whole) {
+                        const float inv = L == 0.f ? 0.f : 1.f / L;
+                        fa *= inv;
+                        fb *= inv;
+                    }
+                    if (rows > (warp & 3) * 32) {  // some row of the warp's
+                        T* dst = static_cast<T*>(a.out) + (int64_t)tok * a.sot + (int64_t)head * a.soh;
+                        float* part = a.part_o + srow * D;
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            float x[16];
+                            uint32_t o[16];
+                            if (ca) tmem_ld16_wait(tO + p * D + c, o);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) x[e] = ca ? __uint_as_float(o[e]) * fa : 0.f;
+                            if (cb) {
+                                tmem_ld16_wait(tO + D + c, o);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) x[e] = fmaf(__uint_as_float(o[e]), fb, x[e]);
+                            }
+                            if (live && whole) {
+#pragma unroll
+                                for (int e = 0; e < 16; e += 8)
+                                    *reinterpret_cast<uint4*>(dst + c + e) =
+                                        make_uint4(Pair<T>::pack(x[e], x[e + 1]), Pair<T>::pack(x[e + 2], x[e + 3]),
+                                                   Pair<T>::pack(x[e + 4], x[e + 5]), Pair<T>::pack(x[e + 6], x[e + 7]));
+                            } else if (live) {
+#pragma unroll
+                                for (int e = 0; e < 16; e += 4)
+                                    *reinterpret_cast<float4*>(part + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                            }
+                        }
+                        if (live && whole && a.lse) a.lse[(int64_t)tok * a.heads + head] = log_sum(M, L);
+                        if (live && !whole) a.part_ml[srow] = make_float2(M, L);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0 && ca) mbar_arrive(&o_free[p]);
+                    if (lane == 0 && cb) mbar_arrive(&o_free[1]);
+                }
+            }
+        } while (next_list(count, false));
     } else {
         regs_inc<REGS_SOFTMAX>();
         constexpr bool CAP = MODE & 1, SLOPE = MODE & 2;
-        // Softmax: warps 0..3 tile A, 4..7 tile B; thread -> query row (TMEM lane), its 128 scores of a unit in registers.
+        // Softmax of pipeline t = warp / 4.
         const int t = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lane_base + t * UNIT, tO = tmem + lane_base + 256 + t * D;
         const float scale2 = a.scale * RAGGED_LOG2E;
         const float cap2 = a.softcap * RAGGED_LOG2E, cap_in = CAP ? 2.f * scale2 / a.softcap : 0.f;
         const float cap_y = CAP ? a.scale / a.softcap : 0.f;  // tanh's argument per unit of raw score
-        uint32_t ucount = 0;
+        uint32_t ucount = 0, icount = 0;
         int count;
         do {
             count = *list_len;
             const int items = abs(count);
-            for (int i = 0; i < items; ++i) {
+            bool ok = true;
+            for (int i = 0; i < items && ok; ++i) {
                 const Item& it = list[i];
-                const int rows = it.n * a.group - it.rt * ROWS - t * TQ;  // valid rows of this tile
-                if (rows <= 0) continue;
-                const int first = it.unit, units = it.end - it.unit;
-                int lo = 0, hi = 0x7fffffff, pos = 0;
+                const int two = it.two, step = two ? 1 : 2;
+                const int begin = it.ub[t], stop = it.ue[t];
+                if (begin >= stop) continue;
+                const int rows = it.n * a.group - it.rt * ROWS - (two ? t * TQ : 0);  // valid rows of the tile
+                const int first = it.unit;
+                // The keys [x, y) the thread's row sees (all, where it is behind the last row), worked out again where a unit
+                // is partly hidden rather than held in registers.
+                auto row_keys = [&]() -> int2 {
+                    if (row >= rows) return make_int2(0, 0x7fffffff);
+                    const int pos = it.pos0 + a.by_group.of(it.rt * ROWS + (two ? t * TQ : 0) + row);
+                    return make_int2(a.window ? max(0, pos - a.window + 1) : 0,
+                                     a.causal ? min(it.len, max(pos + 1, it.prefix)) : it.len);
+                };
+                int pos = 0;
                 float slope = 0.f;
-                if (row < rows) {
-                    const int r = it.rt * ROWS + t * TQ + row;
+                if (SLOPE && row < rows) {
+                    const int r = it.rt * ROWS + (two ? t * TQ : 0) + row;
                     const int tok = a.by_group.of(r);
                     pos = it.pos0 + tok;
-                    hi = a.causal ? min(it.len, max(pos + 1, it.prefix)) : it.len;
-                    lo = a.window ? max(0, pos - a.window + 1) : 0;
-                    if (SLOPE) slope = a.slopes[it.kvh * a.group + r - tok * a.group] * RAGGED_LOG2E;
+                    slope = a.slopes[it.kvh * a.group + r - tok * a.group] * RAGGED_LOG2E;
                 }
-                const int lo_all = __reduce_max_sync(0xffffffffu, lo), hi_all = __reduce_min_sync(0xffffffffu, hi);
+                const bool idle = rows <= (warp & 3) * 32;  // no row of the warp's: it only keeps the barriers' count
+                const int2 keys = row_keys();
+                const int lo_all = __reduce_max_sync(0xffffffffu, keys.x), hi_all = __reduce_min_sync(0xffffffffu, keys.y);
                 // Keys a row may see behind its own position (their distance changes sign): first such key of the warp.
                 const int ahead = SLOPE && (!a.causal || it.prefix > 0)
                                       ? __reduce_min_sync(0xffffffffu, row < rows ? pos : 0x7fffffff)
                                       : 0x7fffffff;
                 float m = -INFINITY, l = 0.f;
-                bool ok = true;
-                for (int j = 0; j < units; ++j, ++ucount) {
+                for (int j = begin; j < stop; j += step, ++ucount) {
                     if (!mbar_wait(&s_full[t], ucount & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE)) {
                         ok = false;
                         break;
                     }
-                    tc_fence_after();
-                    uint32_t v[128];
-                    tmem_ld128_wait(tS, v);
-                    const int key0 = (first + j) * UNIT;
-                    // Finished scores in the base-2 domain, except where the scale is all there is to do (MODE 0).
-                    if (CAP) cap_scores(v, scale2, cap_y, cap_in, cap2);
-                    if (SLOPE) {
-                        const float dist = (float)(pos - key0);  // of key 0
-                        const uint64_t sc = CAP ? pk2(1.f, 1.f) : pk2(scale2, scale2);
-                        if (key0 + UNIT - 1 <= ahead) {
-                            const uint64_t s2 = pk2(slope, slope), b2 = pk2(-slope * dist, -slope * dist);
-#pragma unroll
-                            for (int e = 0; e < 128; e += 2)
-                                put2(v, e, fma2(get2(v, e), sc, fma2(s2, pk2((float)e, (float)(e + 1)), b2)));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 128; ++e)
-                                v[e] = __float_as_uint(fmaf(-slope, fabsf(dist - (float)e),
-                                                            __uint_as_float(v[e]) * (CAP ? 1.f : scale2)));
+                    if (idle) {
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(&p_half[t]);
+                            mbar_arrive(&p_full[t]);
                         }
+                        continue;
                     }
-                    if (key0 < lo_all || key0 + UNIT > hi_all) {
-                        const int l0 = lo - key0, h0 = hi - key0;
+                    tc_fence_after();
+                    const int key0 = (first + j) * UNIT;
+                    const bool part = key0 < lo_all || key0 + UNIT > hi_all;
+                    float mx;
+                    uint32_t v[128];
+                    if (MODE == 0) {
+                        tmem_ld128_wait(tS, v);
+                        if (part) {
+                            const int2 seen_keys = row_keys();
 #pragma unroll
-                        for (int e = 0; e < 128; ++e)
-                            if (e < l0 || e >= h0) v[e] = 0xff800000u;  // -inf
+                            for (int c = 0; c < 4; ++c) {
+                                const uint32_t seen = seen_bits(seen_keys.x, seen_keys.y, key0 + 32 * c);
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (!(seen >> e & 1)) v[32 * c + e] = 0xff800000u;  // -inf
+                            }
+                        }
+                        float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int e = 0; e < 128; e += 8)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                mm[q] = max3(mm[q], __uint_as_float(v[e + 2 * q]), __uint_as_float(v[e + 2 * q + 1]));
+                        mx = max3(mm[0], mm[1], fmaxf(mm[2], mm[3])) * scale2;  // scale2 > 0
+                    } else {
+                        // Cap, bias and mask, 32 scores at a time and back into TMEM as finished scores in the base-2 domain. A
+                        // rolled loop: written out for 128 scores beside the exponentials below, the code was larger than
+                        // the instruction cache next to the scheduler, and a unit took twice as long.
+                        float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        const int2 seen_keys = part ? row_keys() : make_int2(0, 0x7fffffff);
+#pragma unroll 1
+                        for (int c = 0; c < 128; c += 32) {
+                            uint32_t w[32];
+                            tmem_ld32_wait(tS + c, w);
+                            if (CAP) {
+                                float am[2] = {0.f, 0.f};
+#pragma unroll
+                                for (int e = 0; e < 32; e += 4)
+#pragma unroll
+                                    for (int q = 0; q < 2; ++q)
+                                        am[q] = max3(am[q], fabsf(__uint_as_float(w[e + 2 * q])),
+                                                     fabsf(__uint_as_float(w[e + 2 * q + 1])));
+                                // Inside the cap by the polynomial, else by exponential and reciprocal.
+                                if (__all_sync(0xffffffffu, fmaxf(am[0], am[1]) * cap_y <= 1.f)) {
+#pragma unroll
+                                    for (int e = 0; e < 32; e += 2)
+                                        put2(w, e, tanh_poly(mul2(get2(w, e), splat2(cap_y)), cap2));
+                                } else {
+#pragma unroll
+                                    for (int e = 0; e < 32; ++e)
+                                        w[e] = __float_as_uint(capped(__uint_as_float(w[e]) * cap_in, cap2));
+                                }
+                            }
+                            if (SLOPE) {
+                                const float dist = (float)(pos - key0 - c);  // of the chunk's first key
+                                const uint64_t sc = splat2(CAP ? 1.f : scale2);
+                                if (key0 + c + 31 <= ahead) {
+                                    const uint64_t by = splat2(2.f * slope);
+                                    uint64_t b2 = pk2(-slope * dist, slope * (1.f - dist));
+#pragma unroll
+                                    for (int e = 0; e < 32; e += 2) {
+                                        put2(w, e, fma2(get2(w, e), sc, b2));
+                                        b2 = add2(b2, by);
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int e = 0; e < 32; ++e)
+                                        w[e] = __float_as_uint(fmaf(-slope, fabsf(dist - (float)e),
+                                                                    __uint_as_float(w[e]) * (CAP ? 1.f : scale2)));
+                                }
+                            }
+                            if (part) {
+                                const uint32_t seen = seen_bits(seen_keys.x, seen_keys.y, key0 + c);
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (!(seen >> e & 1)) w[e] = 0xff800000u;  // -inf
+                            }
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                                for (int q = 0; q < 4; ++q)
+                                    mm[q] = max3(mm[q], __uint_as_float(w[e + 2 * q]), __uint_as_float(w[e + 2 * q + 1]));
+                            tmem_st32(tS + c, w);
+                        }
+                        mx = max3(mm[0], mm[1], fmaxf(mm[2], mm[3]));
+                        tmem_wait_st();
+                        tmem_ld128_wait(tS, v);
                     }
-                    float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int e = 0; e < 128; e += 8)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            mm[q] = max3(mm[q], __uint_as_float(v[e + 2 * q]), __uint_as_float(v[e + 2 * q + 1]));
-                    float mx = max3(mm[0], mm[1], fmaxf(mm[2], mm[3]));
-                    if (MODE == 0) mx *= scale2;  // scale2 > 0
                     // The maximum moves only when a row's grew by more than 2^8: p stays below 2^8 (inside fp16) and O is
                     // rescaled rarely.
                     if (__any_sync(0xffffffffu, mx > m + 8.f)) {
@@ -625,7 +843,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         const float alpha = m == -INFINITY ? 0.f : ex2_approx(m - mn);
                         m = mn;
                         l *= alpha;
-                        if (j > 0) {
+                        if (j > begin) {
                             // O holds the products of the previous units; they must be complete before the rescale.
                             if (!mbar_wait(&o_done[t], (ucount - 1) & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE)) {
                                 ok = false;
@@ -644,23 +862,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                     // p = 2^(s - m); l sums the fp32 p; P, rounded to the inputs' type (half a step per key, averaged over
                     // the row), goes over the scores already read: 32 scores -> 16 columns.
-                    const uint64_t c2 = MODE ? pk2(1.f, 1.f) : pk2(scale2, scale2);
                     const float nm = m == -INFINITY ? 0.f : -m;
-                    const uint64_t nm2 = pk2(nm, nm);
-                    uint64_t l2 = pk2(0.f, 0.f), l3 = pk2(0.f, 0.f);
+                    const uint64_t nm2 = splat2(nm);
+                    uint64_t l2 = splat2(0.f), l3 = splat2(0.f);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const uint64_t x2 = fma2(get2(v, c * 32 + 2 * e), c2, nm2);
-                            const uint64_t pp = e % POLY_EVERY == POLY_EVERY - 1 ? exp2_poly(x2) : exp2_mufu(x2);
+                            const uint64_t s2 = get2(v, c * 32 + 2 * e);
+                            const float2 x = upk2(MODE == 0 ? fma2(s2, splat2(scale2), nm2) : add2(s2, nm2));
+                            const float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
                             if (e & 1)
-                                l3 = add2(l3, pp);
+                                l3 = add2(l3, pk2(p0, p1));
                             else
-                                l2 = add2(l2, pp);
-                            const float2 p = upk2(pp);
-                            pk[e] = Pair<T>::pack(p.x, p.y);
+                                l2 = add2(l2, pk2(p0, p1));
+                            pk[e] = Pair<T>::pack(p0, p1);
                         }
                         tmem_st16(tS + c * 16, pk);
                         if (c == 1) {
@@ -677,50 +894,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&p_full[t]);
                 }
-                if (!ok || !mbar_wait(&o_done[t], (ucount - 1) & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE)) break;
-                tc_fence_after();
-                const bool live = row < rows;
-                const int r = it.rt * ROWS + t * TQ + row;
-                const int tr = a.by_group.of(r), tok = it.q0 + tr, head = it.kvh * a.group + r - tr * a.group;
-                if (it.slot < 0) {
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    T* dst = static_cast<T*>(a.out) + (int64_t)tok * a.sot + (int64_t)head * a.soh;
-#pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32_wait(tO + c * 32, o);
-                        if (live) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                uint32_t u[4];
-#pragma unroll
-                                for (int z = 0; z < 4; ++z)
-                                    u[z] = Pair<T>::pack(__uint_as_float(o[8 * e + 2 * z]) * inv,
-                                                         __uint_as_float(o[8 * e + 2 * z + 1]) * inv);
-                                *reinterpret_cast<uint4*>(dst + c * 32 + 8 * e) = make_uint4(u[0], u[1], u[2], u[3]);
-                            }
-                        }
-                    }
-                    if (a.lse && live) a.lse[(int64_t)tok * a.heads + head] = log_sum(m, l);
-                } else {
-                    const int64_t srow = (int64_t)it.slot * ROWS + t * TQ + row;
-                    float* dst = a.part_o + srow * D;
-#pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32_wait(tO + c * 32, o);
-                        if (live) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                *reinterpret_cast<uint4*>(dst + c * 32 + 4 * e) =
-                                    make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                        }
-                    }
-                    if (live) a.part_ml[srow] = make_float2(m, l);
-                }
-                tc_fence_before();
+                // m and l to the epilogue, once it has read the pipeline's previous item's.
+                ok = ok && mbar_wait(&o_free[t], (icount & 1) ^ 1, abort_flag, &g_status, B2_DEV_TIMEOUT_EPILOGUE);
+                if (!ok) break;
+                ++icount;
+                ml[t * TQ + row] = make_float2(m, l);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&o_free[t]);
+                if (lane == 0) mbar_arrive(&ml_full[t]);
             }
         } while (next_list(count, false));
     }
