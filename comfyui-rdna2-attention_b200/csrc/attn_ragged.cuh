@@ -24,19 +24,6 @@ namespace b2 {
 
 constexpr float RAGGED_LOG2E = 1.4426950408889634f;
 
-// x / d for 0 <= x < 2^31 and a fixed d, as a product and a shift: with l = ceil(log2 d) and m = floor(2^(31 + l) / d) + 1,
-// x m / 2^(31 + l) exceeds x / d by less than 1 / d.
-struct Divisor {
-    uint32_t m, shift;
-    void set(uint32_t d) {
-        uint32_t l = 0;
-        while ((1ull << l) < d) ++l;
-        m = (uint32_t)((1ull << (31 + l)) / d) + 1;
-        shift = 31 + l;
-    }
-    __device__ __forceinline__ int of(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> shift); }
-};
-
 struct RaggedArgs {
     const void* q;
     int64_t sqt, sqh;

@@ -482,6 +482,19 @@ __device__ __forceinline__ float small_i2f(uint32_t v) {
     return __int_as_float((int)v + 0x4B400000) - 12582912.f;
 }
 
+// x / d for 0 <= x < 2^31 and a fixed d, as a product and a shift: with l = ceil(log2 d) and m = floor(2^(31 + l) / d) + 1,
+// x m / 2^(31 + l) exceeds x / d by less than 1 / d.
+struct Divisor {
+    uint32_t m, shift;
+    void set(uint32_t d) {
+        uint32_t l = 0;
+        while ((1ull << l) < d) ++l;
+        m = (uint32_t)((1ull << (31 + l)) / d) + 1;
+        shift = 31 + l;
+    }
+    __device__ __forceinline__ int of(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> shift); }
+};
+
 // Round-to-nearest-even fp32 -> fp16 and back, never contracted or reordered by the compiler.
 __device__ __forceinline__ float round_h(float x) { return __half2float(__float2half_rn(x)); }
 

@@ -8,9 +8,12 @@
 // has only four bits of the turn's fraction left in 32), sine and cosine of the remainder in 32, and each result is
 // rounded once, to the tensor's type.
 //
-// Bound by HBM: each value is read once and written once. One CTA per token: its F sines and cosines are computed once,
-// into shared memory, and every head's pairs use them. A thread's item is 16 bytes of a's and 16 bytes of b's (both
-// layouts: the same F indices), loaded before the angles are known so that the two latencies overlap.
+// Bound by HBM: each value is read once and written once. A CTA takes one token, or four where there are many: their
+// sines and cosines are computed once, a pair per thread, into shared memory, and every head's pairs use them. A thread's
+// item is 16 bytes of a's and 16 bytes of b's (both layouts: the same F indices), the first one loaded before the angles
+// are known. Measured on 16384 tokens of 32 heads of 128, bf16: 51.4 us, 5.2 TB/s (one token per CTA 59.6, two 55.1,
+// eight 51.4); two items in flight per thread cost more occupancy than they bring (62.5). The bound of six CTAs per SM
+// (40 registers) is the best for the append (63.7 us, 5.3 TB/s, for 15000 tokens of 32 + 2 x 8 heads; eight: 77).
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -40,6 +43,8 @@ struct RopeArgs {
     const float* inv_freq;
     float mscale;
     int tokens, dim, pairs;
+    int items;  // per token
+    Divisor by_items, by_head;
 };
 
 template <class T>
@@ -84,43 +89,29 @@ __device__ __forceinline__ int find_sequence(const int32_t* cu_q, int batch, int
     return (cu_q[lo] <= r && r < cu_q[lo + 1]) ? lo : -1;
 }
 
-template <class T, int V, bool INTER>
-__global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
-    __shared__ float s_cos[MAX_PAIRS], s_sin[MAX_PAIRS];
-    const int t = blockIdx.x;
+constexpr int THREADS = 256;
+
+template <class T, int V, bool INTER, int TOK>
+__global__ void __launch_bounds__(THREADS, 6) rope_kernel(const __grid_constant__ RopeArgs a) {
+    __shared__ float s_cos[TOK][MAX_PAIRS], s_sin[TOK][MAX_PAIRS];
+    __shared__ int64_t s_slot[TOK];  // element offset of the token's cache row; -1: dropped; -2: behind the last sequence
     using W = Vec<T, V>;
+    const int t0 = blockIdx.x * TOK;
     const int per_head = a.dim / (2 * V);
     const int rot_items = a.pairs / V;
-    const int items = (a.heads + 2 * a.kv_heads) * per_head;
-
-    int64_t pos = 0;
-    int64_t slot = -1;
-    if (a.kv_heads) {
-        const int b = find_sequence(a.cu_q, a.batch, t);
-        if (b < 0) return;
-        const int64_t p = (int64_t)a.lengths[b] - a.cu_q[b + 1] + t;
-        pos = p;
-        if (p >= 0) {  // below 2^31: t < cu_q[b + 1]
-            const int pi = (int)p / a.page_size;
-            const int page = pi < a.max_pages ? a.table[(int64_t)b * a.table_ld + pi] : -1;
-            if (page >= 0 && page < a.num_pages) slot = (int64_t)page * a.sc_page + ((int)p - pi * a.page_size) * a.sc_row;
-        }
-        if (slot < 0 && threadIdx.x == 0) atomicOr(&g_status, B2_DEV_BAD_PAGE);
-    }
-    if (a.positions) pos = a.positions[t];
+    const int total = min(TOK, a.tokens - t0) * a.items;
 
     struct Item {
-        const T* src;
-        T* dst;
-        int off_a, off_b, f;
-        bool rotate, live;
+        int tok, head, off_a, off_b, f;
+        bool rotate;
     };
     auto item = [&](int i) {
         Item m;
-        m.live = i < items;
-        if (!m.live) return m;
-        const int head = i / per_head, u = i - head * per_head;
-        m.rotate = u < rot_items && head < a.heads + a.kv_heads;
+        m.tok = TOK == 1 ? 0 : a.by_items.of(i);
+        i -= m.tok * a.items;
+        m.head = a.by_head.of(i);
+        const int u = i - m.head * per_head;
+        m.rotate = u < rot_items && m.head < a.heads + a.kv_heads;
         m.f = u * V;
         if (u < rot_items && !INTER) {
             m.off_a = u * V;
@@ -129,27 +120,23 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
             m.off_a = 2 * u * V;
             m.off_b = m.off_a + V;
         }
-        if (head < a.heads) {
-            m.src = static_cast<const T*>(a.x) + (int64_t)t * a.sxt + head * a.sxh;
-            m.dst = static_cast<T*>(a.out) + (int64_t)t * a.sot + head * a.soh;
-        } else {
-            const bool is_k = head < a.heads + a.kv_heads;
-            const int h = head - a.heads - (is_k ? 0 : a.kv_heads);
-            m.src = is_k ? static_cast<const T*>(a.k) + (int64_t)t * a.skt + h * a.skh
-                         : static_cast<const T*>(a.v) + (int64_t)t * a.svt + h * a.svh;
-            m.dst = static_cast<T*>(is_k ? a.k_cache : a.v_cache) + slot + h * a.sc_head;
-            m.live = slot >= 0;
-        }
         return m;
     };
-    auto load = [](const Item& m, W& wa, W& wb) {
-        if (m.live) {
-            wa = *reinterpret_cast<const W*>(m.src + m.off_a);
-            wb = *reinterpret_cast<const W*>(m.src + m.off_b);
-        }
+    auto load = [&](const Item& m, W& wa, W& wb) {
+        const int64_t t = t0 + m.tok;
+        const T* src;
+        if (m.head < a.heads)
+            src = static_cast<const T*>(a.x) + t * a.sxt + m.head * a.sxh;
+        else if (m.head < a.heads + a.kv_heads)
+            src = static_cast<const T*>(a.k) + t * a.skt + (m.head - a.heads) * a.skh;
+        else
+            src = static_cast<const T*>(a.v) + t * a.svt + (m.head - a.heads - a.kv_heads) * a.svh;
+        wa = *reinterpret_cast<const W*>(src + m.off_a);
+        wb = *reinterpret_cast<const W*>(src + m.off_b);
     };
     auto finish = [&](const Item& m, W& wa, W& wb) {
-        if (!m.live) return;
+        const int64_t t = t0 + m.tok, slot = a.kv_heads ? s_slot[m.tok] : 0;
+        if (slot == -2 || (slot < 0 && m.head >= a.heads)) return;
         if (m.rotate) {
             float x[2 * V];
 #pragma unroll
@@ -159,7 +146,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
             }
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float c = s_cos[m.f + e], s = s_sin[m.f + e];
+                const float c = s_cos[m.tok][m.f + e], s = s_sin[m.tok][m.f + e];
                 const int ia = INTER ? 2 * e : e, ib = INTER ? 2 * e + 1 : V + e;
                 const float p = x[ia], q = x[ib];
                 x[ia] = p * c - q * s;
@@ -171,54 +158,93 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
                 wb.e[e] = from_f<T>(x[V + e]);
             }
         }
-        *reinterpret_cast<W*>(m.dst + m.off_a) = wa;
-        *reinterpret_cast<W*>(m.dst + m.off_b) = wb;
+        T* dst;
+        if (m.head < a.heads)
+            dst = static_cast<T*>(a.out) + t * a.sot + m.head * a.soh;
+        else if (m.head < a.heads + a.kv_heads)
+            dst = static_cast<T*>(a.k_cache) + slot + (m.head - a.heads) * a.sc_head;
+        else
+            dst = static_cast<T*>(a.v_cache) + slot + (m.head - a.heads - a.kv_heads) * a.sc_head;
+        *reinterpret_cast<W*>(dst + m.off_a) = wa;
+        *reinterpret_cast<W*>(dst + m.off_b) = wb;
     };
 
+    Item m;
     W wa, wb;
-    Item m = item(threadIdx.x);
-    load(m, wa, wb);
-    for (int f = threadIdx.x; f < a.pairs; f += blockDim.x) {
-        // turns = p * inv_freq / (2 pi), less its nearest quarter turn: |rest| <= 1/8
-        const double turns = (double)pos * (double)a.inv_freq[f] * 0.15915494309189533577;
-        const double frac = turns - rint(turns);
-        const double quarter = rint(4.0 * frac);
-        const int qn = (int)quarter & 3;
-        float s, c;
-        sincospif((float)(2.0 * (frac - 0.25 * quarter)), &s, &c);
-        const float cc = (qn & 1) ? -s : c, ss = (qn & 1) ? c : s;  // one quarter turn: (cos, sin) -> (-sin, cos)
-        s_cos[f] = ((qn & 2) ? -cc : cc) * a.mscale;
-        s_sin[f] = ((qn & 2) ? -ss : ss) * a.mscale;
-    }
-    __syncthreads();
-    finish(m, wa, wb);
-    for (int i = threadIdx.x + blockDim.x; i < items; i += blockDim.x) {
+    int i = threadIdx.x;
+    if (i < total) {
         m = item(i);
         load(m, wa, wb);
+    }
+    // Each token's position, cache row and angles, by the warps of its share of the CTA.
+    constexpr int SHARE = THREADS / TOK;
+    const int tok = threadIdx.x / SHARE, t = t0 + tok;
+    if (t < a.tokens) {
+        int64_t pos = 0;
+        bool live = true;
+        if (a.kv_heads) {
+            int64_t slot = -1;
+            const int b = find_sequence(a.cu_q, a.batch, t);
+            live = b >= 0;
+            if (live) {
+                pos = (int64_t)a.lengths[b] - a.cu_q[b + 1] + t;
+                if (pos >= 0) {  // below 2^31: t < cu_q[b + 1]
+                    const int pi = (int)pos / a.page_size;
+                    const int page = pi < a.max_pages ? a.table[(int64_t)b * a.table_ld + pi] : -1;
+                    if (page >= 0 && page < a.num_pages)
+                        slot = (int64_t)page * a.sc_page + ((int)pos - pi * a.page_size) * a.sc_row;
+                }
+            }
+            if (threadIdx.x % SHARE == 0) {
+                s_slot[tok] = live ? slot : -2;
+                if (live && slot < 0) atomicOr(&g_status, B2_DEV_BAD_PAGE);
+            }
+        }
+        if (a.positions) pos = a.positions[t];
+        for (int f = threadIdx.x % SHARE; live && f < a.pairs; f += SHARE) {
+            // turns = p * inv_freq / (2 pi), less its nearest quarter turn: |rest| <= 1/8
+            const double turns = (double)pos * (double)a.inv_freq[f] * 0.15915494309189533577;
+            const double frac = turns - rint(turns);
+            const double quarter = rint(4.0 * frac);
+            const int qn = (int)quarter & 3;
+            float s, c;
+            sincospif((float)(2.0 * (frac - 0.25 * quarter)), &s, &c);
+            const float cc = (qn & 1) ? -s : c, ss = (qn & 1) ? c : s;  // one quarter turn: (cos, sin) -> (-sin, cos)
+            s_cos[tok][f] = ((qn & 2) ? -cc : cc) * a.mscale;
+            s_sin[tok][f] = ((qn & 2) ? -ss : ss) * a.mscale;
+        }
+    }
+    __syncthreads();
+    while (i < total) {
         finish(m, wa, wb);
+        i += THREADS;
+        if (i < total) {
+            m = item(i);
+            load(m, wa, wb);
+        }
     }
 }
 
-template <class T>
-int launch(const RopeArgs& a, bool wide, bool inter, cudaStream_t s) {
-    constexpr int V = 16 / sizeof(T);
-    const int items = (a.heads + 2 * a.kv_heads) * (a.dim / (wide ? 2 * V : 2));
-    const int threads = items <= 64 && a.pairs <= 64 ? 64 : items <= 128 ? 128 : 256;
-    if (wide) {
-        if (inter)
-            rope_kernel<T, V, true><<<a.tokens, threads, 0, s>>>(a);
-        else
-            rope_kernel<T, V, false><<<a.tokens, threads, 0, s>>>(a);
-    } else {
-        if (inter)
-            rope_kernel<T, 1, true><<<a.tokens, threads, 0, s>>>(a);
-        else
-            rope_kernel<T, 1, false><<<a.tokens, threads, 0, s>>>(a);
-    }
+template <class T, int V, bool INTER>
+int launch_tok(RopeArgs& a, cudaStream_t s) {
+    a.items = (a.heads + 2 * a.kv_heads) * (a.dim / (2 * V));
+    a.by_items.set(a.items);
+    a.by_head.set(a.dim / (2 * V));
+    if (a.tokens >= 4 * sm_count())
+        rope_kernel<T, V, INTER, 4><<<(a.tokens + 3) / 4, THREADS, 0, s>>>(a);
+    else
+        rope_kernel<T, V, INTER, 1><<<a.tokens, THREADS, 0, s>>>(a);
     return check_launch("rope_kernel");
 }
 
-int run(const RopeArgs& a, int dtype, int inter, void* stream, const char* what) {
+template <class T>
+int launch(RopeArgs& a, bool wide, bool inter, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    if (wide) return inter ? launch_tok<T, V, true>(a, s) : launch_tok<T, V, false>(a, s);
+    return inter ? launch_tok<T, 1, true>(a, s) : launch_tok<T, 1, false>(a, s);
+}
+
+int run(RopeArgs& a, int dtype, int inter, void* stream, const char* what) {
     if (a.dim <= 0 || a.dim % 2 || a.pairs < 0 || 2 * a.pairs > a.dim || a.pairs > MAX_PAIRS)
         return fail(B2_ERR_UNSUPPORTED, "%s: head dim %d with %d rotated pairs (dim even, 2 * pairs <= dim, pairs <= %d)", what,
                     a.dim, a.pairs, MAX_PAIRS);
