@@ -266,14 +266,21 @@ __device__ __forceinline__ void advance(const RaggedArgs& a, Cursor& c, int done
     c.u1 = u.y;
 }
 
-// The descriptor the merge reads: how many of the next CTAs hold the rest of an item that this CTA's run ends inside
-// (`end`: where this run stops in the item), 0 where it does not.
+// How many of the next CTAs hold the rest of an item that this CTA's run ends inside (`end`: where this run stops in the
+// item), 0 where it does not.
 __device__ __forceinline__ int parts_after(const Cursor& c, int end) {
     if (end >= c.u1) return 0;
     const int64_t stop = c.runs.begin(blockIdx.x + 1) + (c.u1 - end);
     int n = 1;
     while (blockIdx.x + 1 + n < c.runs.count && c.runs.begin(blockIdx.x + 1 + n) < stop) ++n;
     return n;
+}
+
+// What the merge reads of an item whose head this CTA holds: parts after the head (below 2^16, as the CTAs are) and rows,
+// q0, kv head, first row.
+template <int ROWS>
+__device__ __forceinline__ int4 describe(const RaggedArgs& a, const Sequence& s, int parts, int kvh, int rt) {
+    return make_int4(parts | min(ROWS, s.n * a.group - rt * ROWS) << 16, s.q0, kvh, rt * ROWS);
 }
 
 // Element offset of a key row of the sequence in k and v (head 0), or -1: behind the last key, or on a page that does
@@ -320,52 +327,60 @@ __device__ __forceinline__ float log_sum(float m2, float l) {
 //   M = max m_p, L = sum l_p 2^(m_p - M), out = sum O_p 2^(m_p - M) / L
 template <class T, int D, int ROWS>
 __global__ void __launch_bounds__(512) merge_kernel(const RaggedArgs a) {
+    pdl_trigger();
     pdl_wait();
     const int x = blockIdx.x, lane = threadIdx.x & 31;
     const int row = blockIdx.y * 16 + (threadIdx.x >> 5);
-    const int4 d = a.desc[x];  // parts after the head, b, kvh, rt
-    if (d.x == 0) return;
-    const Sequence s = load_sequence(a, d.y);
-    const int r = d.w * ROWS + row;
-    if (r >= s.n * a.group) return;
-    const int parts = d.x + 1;
+    const int4 d = a.desc[x];  // parts after the head and rows, q0, kvh, first row: see describe
+    const int parts = (d.x & 0xffff) + 1;
+    if (parts == 1 || row >= d.x >> 16) return;
     auto slot = [&](int p) { return (int64_t)(p == 0 ? 2 * x + 1 : 2 * (x + p)) * ROWS + row; };
-    float M = -INFINITY;
-    for (int p = lane; p < parts; p += 32) M = fmaxf(M, a.part_ml[slot(p)].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float ref = M == -INFINITY ? 0.f : M;
-    constexpr int C = D / 32;
+    constexpr int C = D / 32, BATCH = 8;
     float acc[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) acc[i] = 0.f;
-    float L = 0.f;
+    float M = -INFINITY, L = 0.f;
     for (int p0 = 0; p0 < parts; p0 += 32) {
-        float w = 0.f;
-        if (p0 + lane < parts) {
-            const float2 ml = a.part_ml[slot(p0 + lane)];
-            w = ex2_approx(ml.x - ref);
-            if (w != 0.f) L += w * ml.y;
-        }
+        // 32 parts' (m, l) a lane each, and O of eight of them at a time: the loads do not wait for the weights.
         const int here = min(32, parts - p0);
-#pragma unroll 4
-        for (int p = 0; p < here; ++p) {
-            const float wp = __shfl_sync(0xffffffffu, w, p);
-            if (wp == 0.f) continue;  // a part that saw nothing may hold no O
-            const float* src = a.part_o + slot(p0 + p) * D + lane * C;
-            float v[C];
-            if constexpr (C == 4)
-                *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-            else
-                *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+        const float2 ml = lane < here ? a.part_ml[slot(p0 + lane)] : make_float2(-INFINITY, 0.f);
+        float w = 0.f;
+        for (int b = 0; b < here; b += BATCH) {
+            float v[BATCH][C];
 #pragma unroll
-            for (int i = 0; i < C; ++i) acc[i] = fmaf(wp, v[i], acc[i]);
+            for (int k = 0; k < BATCH; ++k) {
+                const float* src = a.part_o + slot(p0 + min(b + k, here - 1)) * D + lane * C;
+                if constexpr (C == 4)
+                    *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(src);
+                else
+                    *reinterpret_cast<float2*>(v[k]) = *reinterpret_cast<const float2*>(src);
+            }
+            if (b == 0) {
+                float m = fmaxf(M, ml.x);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const float keep = M == -INFINITY ? 0.f : ex2_approx(M - m);
+                M = m;
+                L *= keep;
+#pragma unroll
+                for (int i = 0; i < C; ++i) acc[i] *= keep;
+                w = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M);
+                if (w != 0.f) L += w * ml.y;
+            }
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k) {
+                const float wp = __shfl_sync(0xffffffffu, w, b + k);
+                if (b + k < here && wp != 0.f) {  // a part that saw nothing may hold no O
+#pragma unroll
+                    for (int i = 0; i < C; ++i) acc[i] = fmaf(wp, v[k][i], acc[i]);
+                }
+            }
         }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    const int t = a.by_group.of(r), tok = s.q0 + t, head = d.z * a.group + r - t * a.group;
+    const int r = d.w + row, t = a.by_group.of(r), tok = d.y + t, head = d.z * a.group + r - t * a.group;
     T* dst = static_cast<T*>(a.out) + (int64_t)tok * a.sot + (int64_t)head * a.soh + lane * C;
     uint32_t u[C / 2];
 #pragma unroll
@@ -391,24 +406,6 @@ inline void ragged_slots(RaggedArgs& a, void* workspace, int ctas, int rows, int
     w += (int64_t)ctas * 2 * rows * 8;
     a.desc = reinterpret_cast<int4*>(w);
 }
-// The merge starts while the attention's last CTAs finish (programmatic stream serialization); it reads nothing of
-// theirs before griddepcontrol.wait.
-template <class K>
-int launch_merge(K kernel, const RaggedArgs& a, int ctas, int rows, cudaStream_t s) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas, rows / 16);
-    cfg.blockDim = dim3(512);
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-    if (e != cudaSuccess) return fail(B2_ERR_CUDA, "merge_kernel: %s", cudaGetErrorString(e));
-    return B2_OK;
-}
-
 // The two kernels' launchers (attn_rows.cu, attn_tiles.cu).
 int64_t rows_workspace(int dim);
 int attn_rows(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t s);

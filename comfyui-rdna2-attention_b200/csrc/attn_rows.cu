@@ -72,12 +72,13 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 }
 
 template <class T, int D, bool BIAS>
-__global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const RaggedArgs a) {
+__global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const __grid_constant__ RaggedArgs a) {
     using C = Cfg<D>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int64_t s_run[40];
     __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS];
     pdl_trigger();
+    pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t ring = smem_u32(smem) + warp * C::WARP_BYTES;
     float* o_smem = reinterpret_cast<float*>(smem + warp * C::WARP_BYTES);
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const 
                 if (col == 0) a.part_ml[(int64_t)slot * ROWS + row] = make_float2(M, L);
             }
         }
-        if (c.unit == c.u0) desc = make_int4(parts_after(c, end), c.b, c.kvh, c.rt);
+        if (c.unit == c.u0) desc = describe<ROWS>(a, s, parts_after(c, end), c.kvh, c.rt);
         __syncthreads();  // shared memory is free for the next item
         advance<ROWS, UNIT>(a, c, units);
     }
@@ -315,9 +316,8 @@ int launch_rows(const RaggedArgs& a, cudaStream_t s) {
     static bool done[64] = {false};
     if (int rc = set_smem_once(attn_rows_kernel<T, D, BIAS>, Cfg<D>::SMEM, done)) return rc;
     const int ctas = Cfg<D>::CTAS * sm_count();
-    attn_rows_kernel<T, D, BIAS><<<ctas, THREADS, Cfg<D>::SMEM, s>>>(a);
-    if (int rc = check_launch("attn_rows_kernel")) return rc;
-    return launch_merge(merge_kernel<T, D, ROWS>, a, ctas, ROWS, s);
+    if (int rc = launch_pdl(attn_rows_kernel<T, D, BIAS>, dim3(ctas), THREADS, Cfg<D>::SMEM, s, "attn_rows_kernel", a)) return rc;
+    return launch_pdl(merge_kernel<T, D, ROWS>, dim3(ctas, ROWS / 16), 512, 0, s, "merge_kernel", a);
 }
 
 }  // namespace

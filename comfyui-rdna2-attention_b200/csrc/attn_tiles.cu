@@ -160,7 +160,7 @@ __device__ __forceinline__ int fill_list(const RaggedArgs& a, Cursor* s_cur, Ite
             if (start == u.x && end < u.y) {
                 cur.unit = start;  // for this lane's descriptor only
                 cur.u1 = u.y;
-                a.desc[blockIdx.x] = make_int4(parts_after(cur, end), cur.b, kvh, rt);
+                a.desc[blockIdx.x] = describe<ROWS>(a, cur.s, parts_after(cur, end), kvh, rt);
             }
         }
         const int taken = __popc(__ballot_sync(0xffffffffu, take));
@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
+    pdl_wait();
     // Warp LOAD_WARP lists the CTA's next items; the cursor waits in shared memory meanwhile (it would cost every role's
     // threads twenty registers).
     Cursor* s_cur = reinterpret_cast<Cursor*>(smem + C::OFF_CUR);
@@ -945,9 +946,10 @@ int launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap
     static bool done[64] = {false};
     if (int rc = set_smem_once(attn_tiles_kernel<T, D, MODE, TMA>, Cfg<D>::SMEM, done)) return rc;
     const int ctas = sm_count();
-    attn_tiles_kernel<T, D, MODE, TMA><<<ctas, THREADS, Cfg<D>::SMEM, s>>>(tq, tk, tv, a);
-    if (int rc = check_launch("attn_tiles_kernel")) return rc;
-    return launch_merge(merge_kernel<T, D, ROWS>, a, ctas, ROWS, s);
+    if (int rc = launch_pdl(attn_tiles_kernel<T, D, MODE, TMA>, dim3(ctas), THREADS, Cfg<D>::SMEM, s, "attn_tiles_kernel", tq, tk,
+                            tv, a))
+        return rc;
+    return launch_pdl(merge_kernel<T, D, ROWS>, dim3(ctas, ROWS / 16), 512, 0, s, "merge_kernel", a);
 }
 
 }  // namespace

@@ -61,6 +61,25 @@ inline int set_smem_once(K kernel, int bytes, bool (&done)[64]) {
     return B2_OK;
 }
 
+// Launch with programmatic stream serialization: the kernel may start while the previous one of the stream still runs
+// and reads and writes nothing of others before its griddepcontrol.wait.
+template <class... P>
+inline int launch_pdl(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, const char* name, const P&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e != cudaSuccess) return fail(B2_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+    return B2_OK;
+}
+
 // Per-translation-unit device status words, read and cleared by b2_device_status().
 unsigned int read_status_gemm();
 unsigned int read_status_attention();

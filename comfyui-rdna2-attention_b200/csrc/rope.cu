@@ -93,6 +93,8 @@ constexpr int THREADS = 256;
 
 template <class T, int V, bool INTER, int TOK>
 __global__ void __launch_bounds__(THREADS, 6) rope_kernel(const __grid_constant__ RopeArgs a) {
+    pdl_trigger();
+    pdl_wait();
     __shared__ float s_cos[TOK][MAX_PAIRS], s_sin[TOK][MAX_PAIRS];
     __shared__ int64_t s_slot[TOK];  // element offset of the token's cache row; -1: dropped; -2: behind the last sequence
     using W = Vec<T, V>;
@@ -231,10 +233,8 @@ int launch_tok(RopeArgs& a, cudaStream_t s) {
     a.by_items.set(a.items);
     a.by_head.set(a.dim / (2 * V));
     if (a.tokens >= 4 * sm_count())
-        rope_kernel<T, V, INTER, 4><<<(a.tokens + 3) / 4, THREADS, 0, s>>>(a);
-    else
-        rope_kernel<T, V, INTER, 1><<<a.tokens, THREADS, 0, s>>>(a);
-    return check_launch("rope_kernel");
+        return launch_pdl(rope_kernel<T, V, INTER, 4>, dim3((a.tokens + 3) / 4), THREADS, 0, s, "rope_kernel", a);
+    return launch_pdl(rope_kernel<T, V, INTER, 1>, dim3(a.tokens), THREADS, 0, s, "rope_kernel", a);
 }
 
 template <class T>
