@@ -142,9 +142,13 @@ struct Cursor {
 
 // Finds the CTA's run with all of its threads (THREADS of them; smem: 40 int64). Every thread returns the same cursor.
 template <int ROWS, int UNIT, int THREADS>
-__device__ __forceinline__ Cursor find_run(const RaggedArgs& a, int64_t* smem) {
+__device__ __forceinline__ Cursor find_run(const RaggedArgs& a, int64_t* smem, unsigned int* status) {
     constexpr int WARPS = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // A sequence longer than its row of the table is cut there, and reported.
+    if (a.table && blockIdx.x == 0)
+        for (int b = tid; b < a.batch; b += THREADS)
+            if (a.lengths[b] > (int64_t)a.max_pages * a.page_size) atomicOr(status, B2_DEV_BAD_PAGE);
     auto units_of = [&](int b) -> int64_t {  // every lane of the warp calls it
         return head_units<ROWS, UNIT>(a, b < a.batch ? load_sequence(a, b) : Sequence{}) * a.kv_heads;
     };

@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const 
     const uint32_t ring = smem_u32(smem) + warp * C::WARP_BYTES;
     float* o_smem = reinterpret_cast<float*>(smem + warp * C::WARP_BYTES);
 
-    Cursor c = find_run<ROWS, UNIT, THREADS>(a, s_run);
+    Cursor c = find_run<ROWS, UNIT, THREADS>(a, s_run, &g_status);
     int4 desc = make_int4(0, 0, 0, 0);
     while (c.left > 0) {
         const int end = (int)min((int64_t)c.u1, c.unit + c.left);

@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // threads twenty registers).
     Cursor* s_cur = reinterpret_cast<Cursor*>(smem + C::OFF_CUR);
     {
-        const Cursor found = find_run<ROWS, UNIT, THREADS>(a, reinterpret_cast<int64_t*>(smem + C::OFF_RUN));
+        const Cursor found = find_run<ROWS, UNIT, THREADS>(a, reinterpret_cast<int64_t*>(smem + C::OFF_RUN), &g_status);
         if (threadIdx.x == 0) {
             *s_cur = found;
             a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);

@@ -164,7 +164,7 @@ def test_bad_pages_are_skipped(pkg, dev, rows):
     small = table[:, :4].contiguous()
     out = pkg.ops.attn_paged(q, kc, vc, small, cu, longer, max_q=hint(rows, 2))
     assert torch.equal(out[:2], good[:2])
-    pkg._lib.device_status()
+    assert pkg._lib.device_status() == pkg.ops.BAD_PAGE
 
 
 @pytest.mark.parametrize("rows", ROWS)
@@ -255,3 +255,73 @@ def test_other_stream_and_workspace(pkg, dev):
         got = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, workspace=ws)
     s.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_sequences_share_pages(pkg, dev, rows):
+    """Two sequences whose tables begin with the same pages (a common prompt), the second one longer."""
+    kc, vc, table, _, _ = paged(dev, F16, 2, 128, 16, [0, 0], [64, 100], 13)
+    table[1, :4] = table[0, :4]
+    lengths = torch.tensor([64, 100], dtype=torch.int32, device=dev)
+    fill(kc, vc, table, lengths, 13)
+    q = torch.randn((5, 8, 128), device=dev).half()
+    cu = torch.tensor([0, 2, 5], dtype=torch.int32, device=dev)
+    lse = torch.empty((5, 8), device=dev)
+    out = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, lse=lse, max_q=hint(rows, 4))
+    total = [64, 100]
+    verify(out, lse, q, [2, 3], lambda b: pages_of(kc, table, b, total[b]), lambda b: pages_of(vc, table, b, total[b]), {},
+           None, F16, None)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_cache_offsets_past_32_bits(pkg, dev, rows):
+    """Pages 1.5 * 2^30 elements apart (9.7 GB in all): append, rotation and attention reach them."""
+    step, page, Hk, D = 3 << 29, 16, 1, 64
+    buf = torch.empty(3 * step, dtype=F16, device=dev)
+    cache = lambda at: buf[at:].as_strided((3, page, Hk, D), (step, D, D, 1))
+    kc, vc = cache(0), cache(1 << 20)
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=dev)
+    n = 40
+    x = torch.randn((n, 4, D), device=dev).half()
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    lengths = torch.tensor([n], dtype=torch.int32, device=dev)
+    pkg.ops.kv_append(x[:, 2:3], x[:, 3:], kc, vc, table, cu, lengths)
+    assert torch.equal(pages_of(kc, table, 0, n), x[:, 2:3]) and torch.equal(pages_of(vc, table, 0, n), x[:, 3:])
+    lse = torch.empty((n, 2), device=dev)
+    out = pkg.ops.attn_paged(x[:, :2], kc, vc, table, cu, lengths, lse=lse, max_q=hint(rows, 2))
+    verify(out, lse, x[:, :2], [n], lambda b: x[:, 2:3], lambda b: x[:, 3:], {}, None, F16, None)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_calls_that_overlap(pkg, dev, rows):
+    """Calls on several streams at once, each with its own workspace, give what they give alone."""
+    data = []
+    for i in range(4):
+        kc, vc, table, cu, lengths = paged(dev, F16, 2, 64, 16, [3, 1], [3000 + 100 * i, 50], 20 + i)
+        fill(kc, vc, table, lengths, 20 + i)
+        data.append((torch.randn((4, 4, 64), device=dev).half(), kc, vc, table, cu, lengths))
+    alone = [pkg.ops.attn_paged(*d, max_q=hint(rows, 2)) for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    for _ in range(3):
+        got = []
+        for s, d in zip(streams, data):
+            with torch.cuda.stream(s):
+                got.append(pkg.ops.attn_paged(*d, max_q=hint(rows, 2)))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(alone, got))
+
+
+def test_bound_of_the_cap_on_both_paths(pkg, dev):
+    """Scores across the whole of tanh, small ones beside large ones, so that both ways of computing the cap are taken."""
+    n = 130
+    q = torch.randn((n, 2, 128), device=dev).half()
+    k = torch.randn((400, 1, 128), device=dev).half()
+    k[200:] *= 20
+    v = torch.randn((400, 1, 128), device=dev).half()
+    cu, ck = (torch.tensor([0, x], dtype=torch.int32, device=dev) for x in (n, 400))
+    for cap in (0.5, 8.0, 40.0):
+        for slopes in (None, torch.tensor([0.1, 0.02], device=dev)):
+            out = pkg.ops.attn_packed(q, k, v, cu, ck, softcap=cap, slopes=slopes, max_q=1000)
+            want, _, mass = attend64(q, k, v, softcap=cap, slopes=slopes)
+            attend_check(out, want, mass, F16, 400, v.abs().max().item())
