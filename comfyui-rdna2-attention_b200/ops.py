@@ -612,11 +612,17 @@ def _one_device(t, *others):
     return device
 
 
+def _steps(shape, stride):
+    """Strides with 0 for dimensions of one element, whose stride nothing steps over (torch leaves any value there)."""
+    return tuple([0 if n == 1 else st for n, st in zip(shape, stride)]) if 1 in shape else stride
+
+
 def _packed(t, name, dtype=None):
     """t as [tokens, heads, dim] with a contiguous last dimension (and of the given dtype): its shape and strides."""
     shape, stride = t.shape, t.stride()
     if len(shape) != 3 or (stride[2] != 1 and shape[2] != 1):
         _fail(f"{name} must be [tokens, heads, dim] with a contiguous last dimension")
+    stride = _steps(shape, stride)
     if dtype is not None:
         if t.dtype != dtype:
             _fail(f"{name} has dtype {t.dtype}, needs {dtype}")
@@ -635,7 +641,8 @@ def _cache(k_cache, v_cache, table, kv_heads, dim, dtype, name):
     shape, stride = k_cache.shape, k_cache.stride()
     if len(shape) != 4 or shape[2] != kv_heads or shape[3] != dim or (stride[3] != 1 and dim != 1):
         _fail(f"{name}: k_cache must be [pages, page_size, {kv_heads}, {dim}] with a contiguous last dimension")
-    if v_cache.shape != shape or v_cache.stride() != stride:
+    stride = _steps(shape, stride)
+    if v_cache.shape != shape or _steps(shape, v_cache.stride()) != stride:
         _fail(f"{name}: k_cache and v_cache must have equal shapes and strides")
     if k_cache.dtype != dtype or v_cache.dtype != dtype:
         _fail(f"{name}: k_cache and v_cache must be {dtype} (got {k_cache.dtype}, {v_cache.dtype})")
@@ -836,7 +843,9 @@ def attn_paged(q, k_cache, v_cache, table, cu_q, lengths, scale=None, causal=Tru
     dim^-0.5 unless given): softcap > 0 makes it softcap tanh(s / softcap), slopes (fp32 [heads]) then subtract
     slopes[h] |p - j|. A token that sees no key gets zeros. Rows behind the last sequence are left as they were.
 
-    fp16 or bf16, dim 64 or 128, any group of query heads per KV head, any page size; 16-byte aligned rows. ``lse``
+    fp16 or bf16, dim 64 or 128, any group of query heads per KV head, any page size; 16-byte aligned rows. Positions
+    behind a sequence's end and pages it does not use are never read. Keys and values are multiplied a tile at a time with
+    zero weights where they are hidden, so a NaN or infinity in v reaches the tokens beside those that see it. ``lse``
     (fp32 [tokens, heads]) receives log sum exp(s). ``max_q``, the new tokens of the longest sequence, chooses the kernel
     (default: the mean). ``workspace`` (b2_attn_ragged_workspace_bytes, allocated when not given) must not be shared by
     calls that overlap on the GPU."""

@@ -325,3 +325,19 @@ def test_bound_of_the_cap_on_both_paths(pkg, dev):
             out = pkg.ops.attn_packed(q, k, v, cu, ck, softcap=cap, slopes=slopes, max_q=1000)
             want, _, mass = attend64(q, k, v, softcap=cap, slopes=slopes)
             attend_check(out, want, mass, F16, 400, v.abs().max().item())
+
+
+def test_single_elements_have_no_stride(pkg, dev):
+    """One token, one head, one page of one row: torch's strides of such dimensions mean nothing and may be odd."""
+    buf = torch.randn(4096, device=dev).half()
+    q = buf[:64].as_strided((1, 1, 64), (513, 7, 1))
+    kc = buf[64:128].as_strided((1, 1, 1, 64), (33, 5, 3, 1))
+    vc = buf[128:192].as_strided((1, 1, 1, 64), (9, 11, 13, 1))
+    table = torch.zeros((1, 1), dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    one = torch.ones(1, dtype=torch.int32, device=dev)
+    for rows in ROWS:
+        assert torch.equal(pkg.ops.attn_paged(q, kc, vc, table, cu, one, max_q=rows)[0, 0], vc[0, 0, 0])
+    inv, _ = pkg.ops.rope_frequencies(64, device=dev)
+    pkg.ops.kv_append(q, q, kc, vc, table, cu, one, inv_freq=inv)
+    assert torch.equal(vc[0, 0, 0], q[0, 0]) and torch.equal(kc[0, 0, 0], q[0, 0])  # position 0 does not turn
