@@ -8,6 +8,9 @@
 // their K and V rows with cp.async (16 bytes a lane, rows gathered through the page table; rows behind the last key
 // are zero-filled, so nothing stale reaches a product) into its own ring of stages, and keeps its own maximum, sum and
 // O in registers. No barrier between warps until the item's end, where the four results meet in shared memory.
+//
+// Measured (32 query heads over 8 kv heads of 128): 96 sequences of one token over 500 to 16000 keys, bf16, 460 us, 6.5 TB/s,
+// the copy rate; one token over 1024 keys 9.5 us, the latency of the deal, the page lookup, the keys and the merge.
 #include "attn_ragged.cuh"
 #include "host.hpp"
 

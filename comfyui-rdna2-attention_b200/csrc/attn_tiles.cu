@@ -14,6 +14,10 @@
 //   warp 11           issues the products
 //   warps 12..15      epilogue: O out of TMEM while the softmax warps are at the next item
 // Rows behind a sequence's last key are zero in shared memory, so nothing stale is multiplied.
+//
+// Measured (32 query heads over 8 kv heads of 128, bf16): 2048 tokens over 65 000 keys 1.94 ms, 1106 TFLOP/s, 0.67 of the
+// measured bf16 rate (2.3 ms where the power cap holds the clock near 1.4 GHz); 12 packed documents of 50 to 4000 tokens
+// 577 us, 790 TFLOP/s. A unit takes about 3300 cycles, its four products 2048, a pipeline's softmax 1950.
 #include "attn_ragged.cuh"
 
 namespace b2 {

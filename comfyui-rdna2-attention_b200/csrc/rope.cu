@@ -11,9 +11,9 @@
 // Bound by HBM: each value is read once and written once. A CTA takes one token, or four where there are many: their
 // sines and cosines are computed once, a pair per thread, into shared memory, and every head's pairs use them. A thread's
 // item is 16 bytes of a's and 16 bytes of b's (both layouts: the same F indices), the first one loaded before the angles
-// are known. Measured on 16384 tokens of 32 heads of 128, bf16: 51.4 us, 5.2 TB/s (one token per CTA 59.6, two 55.1,
+// are known. Measured on 16384 tokens of 32 heads of 128, bf16: 50.5 us, 5.3 TB/s (one token per CTA 59.6, two 55.1,
 // eight 51.4); two items in flight per thread cost more occupancy than they bring (62.5). The bound of six CTAs per SM
-// (40 registers) is the best for the append (63.7 us, 5.3 TB/s, for 15000 tokens of 32 + 2 x 8 heads; eight: 77).
+// (40 registers) is the best for the append (58.9 us, 5.7 TB/s, for 15000 tokens of 32 + 2 x 8 heads; eight: 77).
 #include <cuda_bf16.h>
 
 #include "common.cuh"
