@@ -300,52 +300,49 @@ extern "C" int b2_rope(const void* x, int64_t sxt, int64_t sxh, void* out, int64
     return run(a, dtype, interleaved, stream, "rope");
 }
 
-extern "C" int b2_kv_append(const void* k, int64_t skt, int64_t skh, const void* v, int64_t svt, int64_t svh, void* k_cache,
-                            void* v_cache, int64_t s_page, int64_t s_row, int64_t s_head, const int32_t* table, int table_ld,
-                            int max_pages, int num_pages, int page_size, const int32_t* cu_q, const int32_t* lengths,
-                            int batch, const void* q, int64_t sqt, int64_t sqh, void* q_out, int64_t sot, int64_t soh,
-                            const int64_t* positions, const float* inv_freq, float mscale, int tokens, int heads,
-                            int kv_heads, int dim, int pairs, int interleaved, int dtype, void* stream) {
-    if (tokens < 0 || heads < 0 || kv_heads <= 0 || batch < 0 || max_pages < 0 || num_pages < 0 || page_size <= 0 ||
-        table_ld < 0)
+extern "C" int b2_kv_append(const b2_kv_append_args* p, void* stream) {
+    if (!p) return fail(B2_ERR_INVALID, "kv_append: null arguments");
+    if (p->tokens < 0 || p->heads < 0 || p->kv_heads <= 0 || p->batch < 0 || p->max_pages < 0 || p->num_pages < 0 ||
+        p->page_size <= 0 || p->table_ld < 0)
         return fail(B2_ERR_INVALID, "kv_append: bad shape tokens=%d heads=%d kv_heads=%d batch=%d pages %d of %d, page size %d",
-                    tokens, heads, kv_heads, batch, max_pages, num_pages, page_size);
-    if (tokens == 0 || batch == 0) return B2_OK;
-    if (!k || !v || !k_cache || !v_cache || !table || !cu_q || !lengths || (heads && (!q || !q_out)))
+                    p->tokens, p->heads, p->kv_heads, p->batch, p->max_pages, p->num_pages, p->page_size);
+    if (p->tokens == 0 || p->batch == 0) return B2_OK;
+    if (!p->k || !p->v || !p->k_cache || !p->v_cache || !p->table || !p->cu_q || !p->lengths ||
+        (p->heads && (!p->q || !p->q_out)))
         return fail(B2_ERR_INVALID, "kv_append: null pointer");
     RopeArgs a{};
-    a.x = q;
-    a.out = q_out;
-    a.sxt = sqt;
-    a.sxh = sqh;
-    a.sot = sot;
-    a.soh = soh;
-    a.heads = heads;
-    a.k = k;
-    a.v = v;
-    a.k_cache = k_cache;
-    a.v_cache = v_cache;
-    a.skt = skt;
-    a.skh = skh;
-    a.svt = svt;
-    a.svh = svh;
-    a.sc_page = s_page;
-    a.sc_row = s_row;
-    a.sc_head = s_head;
-    a.kv_heads = kv_heads;
-    a.table = table;
-    a.table_ld = table_ld;
-    a.max_pages = max_pages;
-    a.num_pages = num_pages;
-    a.page_size = page_size;
-    a.cu_q = cu_q;
-    a.lengths = lengths;
-    a.batch = batch;
-    a.positions = positions;
-    a.inv_freq = inv_freq;
-    a.mscale = mscale;
-    a.tokens = tokens;
-    a.dim = dim;
-    a.pairs = pairs;
-    return run(a, dtype, interleaved, stream, "kv_append");
+    a.x = p->q;
+    a.out = p->q_out;
+    a.sxt = p->sqt;
+    a.sxh = p->sqh;
+    a.sot = p->sot;
+    a.soh = p->soh;
+    a.heads = p->heads;
+    a.k = p->k;
+    a.v = p->v;
+    a.k_cache = p->k_cache;
+    a.v_cache = p->v_cache;
+    a.skt = p->skt;
+    a.skh = p->skh;
+    a.svt = p->svt;
+    a.svh = p->svh;
+    a.sc_page = p->s_page;
+    a.sc_row = p->s_row;
+    a.sc_head = p->s_head;
+    a.kv_heads = p->kv_heads;
+    a.table = p->table;
+    a.table_ld = p->table_ld;
+    a.max_pages = p->max_pages;
+    a.num_pages = p->num_pages;
+    a.page_size = p->page_size;
+    a.cu_q = p->cu_q;
+    a.lengths = p->lengths;
+    a.batch = p->batch;
+    a.positions = p->positions;
+    a.inv_freq = p->inv_freq;
+    a.mscale = p->mscale;
+    a.tokens = p->tokens;
+    a.dim = p->dim;
+    a.pairs = p->pairs;
+    return run(a, p->dtype, p->interleaved, stream, "kv_append");
 }

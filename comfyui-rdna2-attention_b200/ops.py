@@ -587,6 +587,8 @@ def decode_step(table, x, x2, qkv, att, act, partial, stats, inv_freq, pos, leng
 
 # ---------------------------------------------------------------- rotary positions, paged cache, packed sequences
 _DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_HALF, _BF16, _INT32, _INT64, _FLOAT = torch.float16, torch.bfloat16, torch.int32, torch.int64, torch.float32
+_contiguous = torch.contiguous_format
 MAX_ROPE_PAIRS = 512
 BAD_PAGE = 16  # bit of _lib.device_status(): a page outside the cache was skipped
 
@@ -601,10 +603,10 @@ def _launch(name, device, *args):
 
 
 def _one_device(t, *others):
-    """The index of the one CUDA device that every tensor given is on."""
+    """The index of the one CUDA device that every tensor is on."""
     device = t.get_device()
     for o in others:
-        if o is not None and o.get_device() != device:
+        if o.get_device() != device:
             require_cuda(t, o)
             _fail(f"tensors on {t.device} and {o.device}: one call takes one device")
     if device < 0:
@@ -624,16 +626,16 @@ def _packed(t, name, dtype=None):
         _fail(f"{name} must be [tokens, heads, dim] with a contiguous last dimension")
     stride = _steps(shape, stride)
     if dtype is not None:
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             _fail(f"{name} has dtype {t.dtype}, needs {dtype}")
     elif t.dtype not in _DTYPE_CODES:
         _fail(f"{name} must be fp16, bf16 or fp32 (got {t.dtype})")
     return shape, stride
 
 
-def _ints(t, n, name):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        _fail(f"{name} must be contiguous int32 [{n}] (got {t.dtype}, {tuple(t.shape)})")
+def _ints(t, n, name, what):
+    if t.dtype is not _INT32 or t.shape != (n,) or not t.is_contiguous():
+        _fail(f"{name} {what} must be contiguous int32 [{n}] (got {t.dtype}, {tuple(t.shape)})")
 
 
 def _cache(k_cache, v_cache, table, kv_heads, dim, dtype, name):
@@ -644,14 +646,19 @@ def _cache(k_cache, v_cache, table, kv_heads, dim, dtype, name):
     stride = _steps(shape, stride)
     if v_cache.shape != shape or _steps(shape, v_cache.stride()) != stride:
         _fail(f"{name}: k_cache and v_cache must have equal shapes and strides")
-    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         _fail(f"{name}: k_cache and v_cache must be {dtype} (got {k_cache.dtype}, {v_cache.dtype})")
     if shape[1] == 0:
         _fail(f"{name}: pages of no rows")
     tshape, tstride = table.shape, table.stride()
-    if table.dtype != torch.int32 or len(tshape) != 2 or (tstride[1] != 1 and tshape[1] > 1):
+    if table.dtype is not _INT32 or len(tshape) != 2 or (tstride[1] != 1 and tshape[1] > 1):
         _fail(f"{name}: the page table must be int32 [batch, pages] with contiguous rows")
     return shape, stride, tshape, tstride
+
+
+# The argument blocks of the C entry points: pointers and strides, then sizes, then factors.
+_APPEND = struct.Struct("=QqqQqqQQqqqQQQQqqQqqQQ12if")  # b2_kv_append_args
+_RAGGED = struct.Struct("=QqqQqqQQQqqqQQQQQQ14i2f")  # b2_attn_ragged_args
 
 
 def rope_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_length=None, slow=1.0, fast=32.0, device=None):
@@ -691,7 +698,7 @@ def _pairs(inv_freq, dim, name):
         _fail(f"{name}: head dim {dim} must be even")
     if inv_freq is None:
         return 0
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+    if inv_freq.dtype is not _FLOAT or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         _fail(f"{name}: inv_freq must be contiguous fp32 [pairs]")
     pairs = inv_freq.shape[0]
     if 2 * pairs > dim or pairs > MAX_ROPE_PAIRS:
@@ -700,7 +707,7 @@ def _pairs(inv_freq, dim, name):
 
 
 def _positions(t, tokens, name):
-    if t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != tokens or not t.is_contiguous():
+    if t.dtype is not _INT64 or t.shape != (tokens,) or not t.is_contiguous():
         _fail(f"{name}: positions must be contiguous int64 [{tokens}] (got {t.dtype}, {tuple(t.shape)})")
 
 
@@ -714,7 +721,7 @@ def rope(x, positions, inv_freq, interleaved=False, mscale=1.0, out=None):
     pairs = _pairs(inv_freq, dim, "rope")
     _positions(positions, tokens, "rope")
     if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        out = torch.empty_like(x, memory_format=_contiguous)
         so = out.stride()
     else:
         oshape, so = _packed(out, "rope output", x.dtype)
@@ -745,8 +752,8 @@ def kv_append(k, v, k_cache, v_cache, table, cu_q, lengths, inv_freq=None, q=Non
         _fail(f"kv_append k and v must have equal shapes [tokens, kv_heads, dim] (got {tuple(shape)}, {tuple(vshape)})")
     cshape, sc, tshape, st = _cache(k_cache, v_cache, table, kv_heads, dim, dtype, "kv_append")
     batch = tshape[0]
-    _ints(cu_q, batch + 1, "kv_append cu_q")
-    _ints(lengths, batch, "kv_append lengths")
+    _ints(cu_q, batch + 1, "kv_append", "cu_q")
+    _ints(lengths, batch, "kv_append", "lengths")
     pairs = _pairs(inv_freq, dim, "kv_append")
     if positions is not None:
         _positions(positions, tokens, "kv_append")
@@ -757,7 +764,7 @@ def kv_append(k, v, k_cache, v_cache, table, cu_q, lengths, inv_freq=None, q=Non
         if qshape[0] != tokens or qshape[2] != dim:
             _fail(f"kv_append q must be [{tokens}, heads, {dim}] (got {tuple(qshape)})")
         if q_out is None:
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            q_out = torch.empty_like(q, memory_format=_contiguous)
             so = q_out.stride()
         else:
             oshape, so = _packed(q_out, "kv_append q_out", dtype)
@@ -765,17 +772,15 @@ def kv_append(k, v, k_cache, v_cache, table, cu_q, lengths, inv_freq=None, q=Non
                 _fail(f"kv_append q_out has shape {tuple(oshape)}, q {tuple(qshape)}")
     elif q_out is not None:
         _fail("kv_append: q_out without q")
-    device = _one_device(k, v, k_cache, v_cache, table, cu_q, lengths, inv_freq, positions, q, q_out)
-    _launch("b2_kv_append", device, k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], k_cache.data_ptr(),
-            v_cache.data_ptr(), sc[0], sc[1], sc[2], table.data_ptr(), st[0], tshape[1], cshape[0], cshape[1],
-            cu_q.data_ptr(), lengths.data_ptr(), batch, q.data_ptr() if heads else None, sq[0], sq[1],
-            q_out.data_ptr() if heads else None, so[0], so[1], positions.data_ptr() if positions is not None else None,
-            inv_freq.data_ptr() if pairs else None, mscale, tokens, heads, kv_heads, dim, pairs, 1 if interleaved else 0,
-            _DTYPE_CODES[dtype])
+    device = _one_device(k, v, k_cache, v_cache, table, cu_q, lengths, *[t for t in (inv_freq, positions, q, q_out)
+                                                                         if t is not None])
+    _launch("b2_kv_append", device, _APPEND.pack(
+        k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], k_cache.data_ptr(), v_cache.data_ptr(), sc[0], sc[1], sc[2],
+        table.data_ptr(), cu_q.data_ptr(), lengths.data_ptr(), q.data_ptr() if heads else 0, sq[0], sq[1],
+        q_out.data_ptr() if heads else 0, so[0], so[1], 0 if positions is None else positions.data_ptr(),
+        inv_freq.data_ptr() if pairs else 0, st[0], tshape[1], cshape[0], cshape[1], batch, tokens, heads, kv_heads, dim, pairs,
+        1 if interleaved else 0, _DTYPE_CODES[dtype], mscale))
     return q_out
-
-
-_RAGGED = struct.Struct("=QqqQqqQQQqqqQQQQQQ14i2f")  # b2_attn_ragged_args
 
 
 def _attn_ragged(name, q, qshape, sq, k, v, sk, kv_heads, table, table_dims, cu_q, lengths, batch, scale, causal, softcap,
@@ -784,37 +789,43 @@ def _attn_ragged(name, q, qshape, sq, k, v, sk, kv_heads, table, table_dims, cu_
     head) and table_dims = (row stride, pages per sequence, pages, page size), or packed rows without a table)."""
     tokens, heads, dim = qshape
     dtype = q.dtype
-    if dtype != torch.float16 and dtype != torch.bfloat16:
+    if dtype is not _HALF and dtype is not _BF16:
         _fail(f"{name}: q must be fp16 or bf16 (got {dtype})")
     if dim != 64 and dim != 128:
         _fail(f"{name}: head dim {dim} (64 or 128)")
     if kv_heads == 0 or heads == 0 or heads % kv_heads:
         _fail(f"{name}: {heads} query heads do not group over {kv_heads} KV heads")
-    _ints(cu_q, batch + 1, name + " cu_q")
+    _ints(cu_q, batch + 1, name, "cu_q")
+    given = []
     if prefix is not None:
-        _ints(prefix, batch, name + " prefix")
-    if slopes is not None and (slopes.dtype != torch.float32 or slopes.dim() != 1 or slopes.shape[0] != heads
-                               or not slopes.is_contiguous()):
-        _fail(f"{name} slopes must be contiguous fp32 [{heads}]")
+        _ints(prefix, batch, name, "prefix")
+        given.append(prefix)
+    if slopes is not None:
+        if slopes.dtype is not _FLOAT or slopes.shape != (heads,) or not slopes.is_contiguous():
+            _fail(f"{name} slopes must be contiguous fp32 [{heads}]")
+        given.append(slopes)
     scale = dim ** -0.5 if scale is None else float(scale)
     if not 0 < scale < 3e38 or not 0 <= softcap < 3e38 or window < 0:
         _fail(f"{name}: scale {scale} must be positive, softcap {softcap} and window {window} not negative")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = torch.empty_like(q, memory_format=_contiguous)
         so = out.stride()
     else:
         oshape, so = _packed(out, name + " output", dtype)
         if oshape != qshape:
             _fail(f"{name} output has shape {tuple(oshape)}, q {tuple(qshape)}")
-    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (tokens, heads) or not lse.is_contiguous()):
-        _fail(f"{name} lse must be contiguous fp32 [{tokens}, {heads}]")
+        given.append(out)
+    if lse is not None:
+        if lse.dtype is not _FLOAT or lse.shape != (tokens, heads) or not lse.is_contiguous():
+            _fail(f"{name} lse must be contiguous fp32 [{tokens}, {heads}]")
+        given.append(lse)
+    if table is not None:
+        given.append(table)
+    if workspace is not None:
+        given.append(workspace)
     max_q = -(-tokens // max(batch, 1)) if max_q is None else min(max(int(max_q), 0), 1 << 30)
-    device = _one_device(q, k, v, table, cu_q, lengths, prefix, slopes, out, lse, workspace)
-    if device == torch._C._cuda_getDevice():
-        nbytes = _ragged_workspace(heads, kv_heads, dim, max_q)
-    else:
-        with torch.cuda.device(device):
-            nbytes = _ragged_workspace(heads, kv_heads, dim, max_q)
+    device = _one_device(q, k, v, cu_q, lengths, *given)
+    nbytes = _ragged_workspace(device, heads, kv_heads, dim, max_q)
     if workspace is None:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < nbytes:
@@ -831,8 +842,21 @@ def _attn_ragged(name, q, qshape, sq, k, v, sk, kv_heads, table, table_dims, cu_
     return out
 
 
-def _ragged_workspace(*args):
-    return _lib.load().b2_attn_ragged_workspace_bytes(*args)
+_workspace_sizes = {}  # (device, heads, kv heads, dim, max_q) -> bytes: the sizes depend on nothing else
+
+
+def _ragged_workspace(*key):
+    nbytes = _workspace_sizes.get(key)
+    if nbytes is None:
+        if len(_workspace_sizes) >= 4096:
+            _workspace_sizes.clear()
+        if key[0] == torch._C._cuda_getDevice():
+            nbytes = _lib.load().b2_attn_ragged_workspace_bytes(*key[1:])
+        else:
+            with torch.cuda.device(key[0]):
+                nbytes = _lib.load().b2_attn_ragged_workspace_bytes(*key[1:])
+        _workspace_sizes[key] = nbytes
+    return nbytes
 
 
 def attn_paged(q, k_cache, v_cache, table, cu_q, lengths, scale=None, causal=True, softcap=0.0, window=0, slopes=None,
@@ -855,7 +879,7 @@ def attn_paged(q, k_cache, v_cache, table, cu_q, lengths, scale=None, causal=Tru
     kv_heads = k_cache.shape[2]
     cshape, sc, tshape, st = _cache(k_cache, v_cache, table, kv_heads, qshape[2], q.dtype, "attn_paged")
     batch = tshape[0]
-    _ints(lengths, batch, "attn_paged lengths")
+    _ints(lengths, batch, "attn_paged", "lengths")
     return _attn_ragged("attn_paged", q, qshape, sq, k_cache, v_cache, sc[:3], kv_heads, table,
                         (st[0], tshape[1], cshape[0], cshape[1]), cu_q, lengths, batch, scale, causal, softcap, window, slopes,
                         prefix, max_q, out, lse, workspace)
@@ -874,7 +898,7 @@ def attn_packed(q, k, v, cu_q, cu_k, scale=None, causal=True, softcap=0.0, windo
     if cu_q.dim() != 1 or cu_q.shape[0] < 1:
         _fail("attn_packed cu_q must be int32 [batch + 1]")
     batch = cu_q.shape[0] - 1
-    _ints(cu_k, batch + 1, "attn_packed cu_k")
+    _ints(cu_k, batch + 1, "attn_packed", "cu_k")
     return _attn_ragged("attn_packed", q, qshape, sq, k, v, (0, sk[0], sk[1]), kshape[1], None, (0, 0, 0, 0), cu_q, cu_k, batch, scale,
                         causal, softcap, window, slopes, prefix, max_q, out, lse, workspace)
 

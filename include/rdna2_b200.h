@@ -286,12 +286,27 @@ int b2_rope(const void* x, int64_t sxt, int64_t sxh, void* out, int64_t sot, int
 /* New keys and values into the cache: k [tokens, kv_heads, dim] rotated as b2_rope does (pairs 0: as it is) and v as it
  * is go to their positions lengths[b] - n_b + i; with heads > 0, q is rotated into q_out (which may be q) in the same
  * launch. The angles use the cache positions, or positions[t] where given. */
-int b2_kv_append(const void* k, int64_t skt, int64_t skh, const void* v, int64_t svt, int64_t svh, void* k_cache,
-                 void* v_cache, int64_t s_page, int64_t s_row, int64_t s_head, const int32_t* table, int table_ld,
-                 int max_pages, int num_pages, int page_size, const int32_t* cu_q, const int32_t* lengths, int batch,
-                 const void* q, int64_t sqt, int64_t sqh, void* q_out, int64_t sot, int64_t soh, const int64_t* positions,
-                 const float* inv_freq, float mscale, int tokens, int heads, int kv_heads, int dim, int pairs,
-                 int interleaved, int dtype, void* stream);
+typedef struct b2_kv_append_args {
+    const void* k;
+    int64_t skt, skh; /* element strides: token, head */
+    const void* v;
+    int64_t svt, svh;
+    void* k_cache;
+    void* v_cache;
+    int64_t s_page, s_row, s_head;
+    const int32_t* table;
+    const int32_t* cu_q;
+    const int32_t* lengths;
+    const void* q; /* with heads 0: null */
+    int64_t sqt, sqh;
+    void* q_out;
+    int64_t sot, soh;
+    const int64_t* positions; /* int64 [tokens], or null */
+    const float* inv_freq;
+    int table_ld, max_pages, num_pages, page_size, batch, tokens, heads, kv_heads, dim, pairs, interleaved, dtype;
+    float mscale;
+} b2_kv_append_args;
+int b2_kv_append(const b2_kv_append_args* args, void* stream);
 /* Attention of packed sequences' new tokens. Token i of sequence b sits at position pos = len - n + i of its len keys
  * and sees key j where (not causal or j <= pos or j < prefix[b]) and (window == 0 or pos - j < window):
  *   s = scale q.k;  s = softcap tanh(s / softcap) if softcap > 0;  s -= slopes[h] |pos - j| if slopes;

@@ -147,10 +147,14 @@ def test_c_entry_points_check_before_launching(pkg):
                                                                           dim, pairs, 0, dtype, P(None))
     assert [rope(x=P(None)), rope(tokens=-1), rope(dim=63), rope(pairs=33), rope(dim=2048, pairs=1000), rope(dtype=3),
             rope(tokens=0)] == [1, 1, 2, 2, 2, 2, 0]
-    app = lambda k=fake, page=16, heads=0, batch=2: lib.b2_kv_append(
-        k, 64, 64, fake, 64, 64, fake, fake, 1024, 64, 64, fake, 3, 3, 6, page, fake, fake, batch, P(None), 0, 0, P(None), 0, 0,
-        P(None), fake, 1.0, 4, heads, 1, 64, 32, 0, 0, P(None))
-    assert [app(k=P(None)), app(page=0), app(heads=2), app(batch=0)] == [1, 1, 1, 0]
+    block = dict(k=4096, skt=64, skh=64, v=4096, svt=64, svh=64, k_cache=4096, v_cache=4096, s_page=1024, s_row=64, s_head=64,
+                 table=4096, cu_q=4096, lengths=4096, q=0, sqt=0, sqh=0, q_out=0, sot=0, soh=0, positions=0, inv_freq=4096,
+                 table_ld=3, max_pages=3, num_pages=6, page_size=16, batch=2, tokens=4, heads=0, kv_heads=1, dim=64, pairs=32,
+                 interleaved=0, dtype=0, mscale=1.0)
+    app = lambda **kw: lib.b2_kv_append(pkg.ops._APPEND.pack(*{**block, **kw}.values()), P(None))
+    assert lib.b2_kv_append(None, P(None)) == 1
+    assert [app(k=0), app(page_size=0), app(heads=2), app(kv_heads=0), app(batch=0), app(tokens=0), app(dim=63), app(dtype=3),
+            app(pairs=33)] == [1, 1, 1, 1, 0, 0, 2, 2, 2]
 
 
 def test_rope_frequencies(pkg):
