@@ -55,7 +55,7 @@ SIGNATURES = {
     "b2_attn_decode_noalloc": (I, [P, P, P, P, P, I, I, I, I, F, P]),
     "b2_decode_step": (I, [P, I, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, F, ctypes.c_longlong, P]),
     "b2_decode_step_splits": (I, [I]),
-    "b2_rope": (I, [P, I64, I64, P, I64, I64, P, P, F, I, I, I, I, I, I, P]),
+    "b2_rope": (I, [P, P]),
     "b2_kv_append": (I, [P, P]),
     "b2_attn_ragged_workspace_bytes": (I64, [I, I, I, I]),
     "b2_attn_ragged": (I, [P, P]),

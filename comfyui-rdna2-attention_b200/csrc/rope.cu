@@ -277,27 +277,26 @@ unsigned int read_status_rope() {
 
 using namespace b2;
 
-extern "C" int b2_rope(const void* x, int64_t sxt, int64_t sxh, void* out, int64_t sot, int64_t soh,
-                       const int64_t* positions, const float* inv_freq, float mscale, int tokens, int heads, int dim,
-                       int pairs, int interleaved, int dtype, void* stream) {
-    if (tokens < 0 || heads < 0) return fail(B2_ERR_INVALID, "rope: bad shape tokens=%d heads=%d", tokens, heads);
-    if (tokens == 0 || heads == 0) return B2_OK;
-    if (!x || !out || !positions) return fail(B2_ERR_INVALID, "rope: null pointer");
+extern "C" int b2_rope(const b2_rope_args* p, void* stream) {
+    if (!p) return fail(B2_ERR_INVALID, "rope: null arguments");
+    if (p->tokens < 0 || p->heads < 0) return fail(B2_ERR_INVALID, "rope: bad shape tokens=%d heads=%d", p->tokens, p->heads);
+    if (p->tokens == 0 || p->heads == 0) return B2_OK;
+    if (!p->x || !p->out || !p->positions) return fail(B2_ERR_INVALID, "rope: null pointer");
     RopeArgs a{};
-    a.x = x;
-    a.out = out;
-    a.sxt = sxt;
-    a.sxh = sxh;
-    a.sot = sot;
-    a.soh = soh;
-    a.heads = heads;
-    a.positions = positions;
-    a.inv_freq = inv_freq;
-    a.mscale = mscale;
-    a.tokens = tokens;
-    a.dim = dim;
-    a.pairs = pairs;
-    return run(a, dtype, interleaved, stream, "rope");
+    a.x = p->x;
+    a.out = p->out;
+    a.sxt = p->sxt;
+    a.sxh = p->sxh;
+    a.sot = p->sot;
+    a.soh = p->soh;
+    a.heads = p->heads;
+    a.positions = p->positions;
+    a.inv_freq = p->inv_freq;
+    a.mscale = p->mscale;
+    a.tokens = p->tokens;
+    a.dim = p->dim;
+    a.pairs = p->pairs;
+    return run(a, p->dtype, p->interleaved, stream, "rope");
 }
 
 extern "C" int b2_kv_append(const b2_kv_append_args* p, void* stream) {

@@ -657,6 +657,7 @@ def _cache(k_cache, v_cache, table, kv_heads, dim, dtype, name):
 
 
 # The argument blocks of the C entry points: pointers and strides, then sizes, then factors.
+_ROPE = struct.Struct("=QqqQqqQQ6if")  # b2_rope_args
 _APPEND = struct.Struct("=QqqQqqQQqqqQQQQqqQqqQQ12if")  # b2_kv_append_args
 _RAGGED = struct.Struct("=QqqQqqQQQqqqQQQQQQ14i2f")  # b2_attn_ragged_args
 
@@ -728,8 +729,9 @@ def rope(x, positions, inv_freq, interleaved=False, mscale=1.0, out=None):
         if oshape != shape:
             _fail(f"rope output has shape {tuple(oshape)}, x {tuple(shape)}")
     device = _one_device(x, positions, inv_freq, out)
-    _launch("b2_rope", device, x.data_ptr(), sx[0], sx[1], out.data_ptr(), so[0], so[1], positions.data_ptr(),
-            inv_freq.data_ptr(), mscale, tokens, heads, dim, pairs, 1 if interleaved else 0, _DTYPE_CODES[x.dtype])
+    _launch("b2_rope", device, _ROPE.pack(
+        x.data_ptr(), sx[0], sx[1], out.data_ptr(), so[0], so[1], positions.data_ptr(), inv_freq.data_ptr(), tokens, heads, dim,
+        pairs, 1 if interleaved else 0, _DTYPE_CODES[x.dtype], mscale))
     return out
 
 

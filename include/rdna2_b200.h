@@ -280,9 +280,17 @@ int b2_attn_decode_noalloc(const float* q, const float* k, const float* v, const
  * interleaved; the other values are copied. Element strides sxt, sxh (token, head) of x and sot, soh of out, the last
  * dimension contiguous; out may be x. positions int64 (negative ones turn back), inv_freq fp32 [pairs]; dim even,
  * 2 * pairs <= dim, pairs <= 512; dtype any of the three. */
-int b2_rope(const void* x, int64_t sxt, int64_t sxh, void* out, int64_t sot, int64_t soh, const int64_t* positions,
-            const float* inv_freq, float mscale, int tokens, int heads, int dim, int pairs, int interleaved, int dtype,
-            void* stream);
+typedef struct b2_rope_args {
+    const void* x;
+    int64_t sxt, sxh;
+    void* out;
+    int64_t sot, soh;
+    const int64_t* positions;
+    const float* inv_freq;
+    int tokens, heads, dim, pairs, interleaved, dtype;
+    float mscale;
+} b2_rope_args;
+int b2_rope(const b2_rope_args* args, void* stream);
 /* New keys and values into the cache: k [tokens, kv_heads, dim] rotated as b2_rope does (pairs 0: as it is) and v as it
  * is go to their positions lengths[b] - n_b + i; with heads > 0, q is rotated into q_out (which may be q) in the same
  * launch. The angles use the cache positions, or positions[t] where given. */

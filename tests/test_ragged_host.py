@@ -143,10 +143,12 @@ def test_c_entry_points_check_before_launching(pkg):
     assert status(batch=0) == 0 and status(tokens=0) == 0
     assert lib.b2_attn_ragged(None, P(None)) == 1
     assert lib.b2_attn_ragged_workspace_bytes(8, 2, 96, 1) == 0 and lib.b2_attn_ragged_workspace_bytes(8, 2, 128, 1) > 0
-    rope = lambda x=fake, tokens=4, dim=64, pairs=32, dtype=0: lib.b2_rope(x, 64, 64, fake, 64, 64, fake, fake, 1.0, tokens, 1,
-                                                                          dim, pairs, 0, dtype, P(None))
-    assert [rope(x=P(None)), rope(tokens=-1), rope(dim=63), rope(pairs=33), rope(dim=2048, pairs=1000), rope(dtype=3),
-            rope(tokens=0)] == [1, 1, 2, 2, 2, 2, 0]
+    turn = dict(x=4096, sxt=64, sxh=64, out=4096, sot=64, soh=64, positions=4096, inv_freq=4096, tokens=4, heads=1, dim=64,
+                pairs=32, interleaved=0, dtype=0, mscale=1.0)
+    rope = lambda **kw: lib.b2_rope(pkg.ops._ROPE.pack(*{**turn, **kw}.values()), P(None))
+    assert [rope(x=0), rope(tokens=-1), rope(dim=63), rope(pairs=33), rope(dim=2048, pairs=1000), rope(dtype=3),
+            rope(positions=0), rope(inv_freq=0), rope(tokens=0)] == [1, 1, 2, 2, 2, 2, 1, 1, 0]
+    assert lib.b2_rope(None, P(None)) == 1
     block = dict(k=4096, skt=64, skh=64, v=4096, svt=64, svh=64, k_cache=4096, v_cache=4096, s_page=1024, s_row=64, s_head=64,
                  table=4096, cu_q=4096, lengths=4096, q=0, sqt=0, sqh=0, q_out=0, sot=0, soh=0, positions=0, inv_freq=4096,
                  table_ld=3, max_pages=3, num_pages=6, page_size=16, batch=2, tokens=4, heads=0, kv_heads=1, dim=64, pairs=32,
