@@ -61,7 +61,7 @@ __device__ __forceinline__ Sequence load_sequence(const RaggedArgs& a, int b) {
     s.n = max(min(a.cu_q[b + 1], a.tokens) - s.q0, 0);
     s.key0 = 0;
     if (a.table) {
-        s.len = max(a.lengths[b], 0);
+        s.len = min(max(a.lengths[b], 0), 1 << 30);  // so that positions and units keep to 32 bits
         s.len = (int)min((int64_t)s.len, (int64_t)a.max_pages * a.page_size);  // no key lies behind the table
     } else {
         const int k0 = min(max(a.lengths[b], 0), a.key_rows);

@@ -719,6 +719,8 @@ def rope(x, positions, inv_freq, interleaved=False, mscale=1.0, out=None):
     gradient of a rotation is the rotation by -positions). ``out`` may be x itself, but not overlap it otherwise."""
     shape, sx = _packed(x, "rope x")
     tokens, heads, dim = shape
+    if inv_freq is None:
+        _fail("rope needs inv_freq (fp32 [pairs], see rope_frequencies)")
     pairs = _pairs(inv_freq, dim, "rope")
     _positions(positions, tokens, "rope")
     if out is None:

@@ -103,6 +103,8 @@ def test_rope_and_packed_refuse(pkg, calls):
               (torch.zeros(5, 2, 63), pos, inv[:8]), (torch.zeros(1, 1, 2048), pos[:1], torch.zeros(600))):
         with pytest.raises(RuntimeError):
             ops.rope(*a)
+    with pytest.raises(RuntimeError, match="inv_freq"):
+        ops.rope(x, pos, None)
     with pytest.raises(RuntimeError, match="output"):
         ops.rope(x, pos, inv, out=torch.zeros(5, 2, 32))
     q, k, cu = torch.zeros(5, 4, 64, dtype=H16), torch.zeros(7, 2, 64, dtype=H16), torch.zeros(3, dtype=torch.int32)
