@@ -593,13 +593,21 @@ MAX_ROPE_PAIRS = 512
 BAD_PAGE = 16  # bit of _lib.device_status(): a page outside the cache was skipped
 
 
-def _launch(name, device, *args):
-    """call() with ``device`` (its index) current, on torch's current stream of it."""
+_entries = {}  # name -> the library's function
+
+
+def _launch(name, device, block):
+    """The entry point ``name`` with its argument block, on torch's current stream of ``device`` (an index)."""
+    entry = _entries.get(name)
+    if entry is None:
+        entry = _entries[name] = getattr(_lib.load(), name)
     if device == torch._C._cuda_getDevice():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+        status = entry(block, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+            status = entry(block, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        _lib.check(status, name)
 
 
 def _one_device(t, *others):
@@ -641,8 +649,8 @@ def _ints(t, n, name, what):
 def _cache(k_cache, v_cache, table, kv_heads, dim, dtype, name):
     """The checks of a paged cache and its table; the cache's shape and strides and the table's."""
     shape, stride = k_cache.shape, k_cache.stride()
-    if len(shape) != 4 or shape[2] != kv_heads or shape[3] != dim or (stride[3] != 1 and dim != 1):
-        _fail(f"{name}: k_cache must be [pages, page_size, {kv_heads}, {dim}] with a contiguous last dimension")
+    if len(shape) != 4 or shape[3] != dim or (stride[3] != 1 and dim != 1) or (kv_heads is not None and shape[2] != kv_heads):
+        _fail(f"{name}: k_cache must be [pages, page_size, {kv_heads or 'kv_heads'}, {dim}] with a contiguous last dimension")
     stride = _steps(shape, stride)
     if v_cache.shape != shape or _steps(shape, v_cache.stride()) != stride:
         _fail(f"{name}: k_cache and v_cache must have equal shapes and strides")
@@ -808,7 +816,7 @@ def _attn_ragged(name, q, qshape, sq, k, v, sk, kv_heads, table, table_dims, cu_
         if slopes.dtype is not _FLOAT or slopes.shape != (heads,) or not slopes.is_contiguous():
             _fail(f"{name} slopes must be contiguous fp32 [{heads}]")
         given.append(slopes)
-    scale = dim ** -0.5 if scale is None else float(scale)
+    scale = (0.125 if dim == 64 else 128 ** -0.5) if scale is None else float(scale)
     if not 0 < scale < 3e38 or not 0 <= softcap < 3e38 or window < 0:
         _fail(f"{name}: scale {scale} must be positive, softcap {softcap} and window {window} not negative")
     if out is None:
@@ -878,10 +886,8 @@ def attn_paged(q, k_cache, v_cache, table, cu_q, lengths, scale=None, causal=Tru
     (default: the mean). ``workspace`` (b2_attn_ragged_workspace_bytes, allocated when not given) must not be shared by
     calls that overlap on the GPU."""
     qshape, sq = _packed(q, "attn_paged q")
-    if k_cache.dim() != 4:
-        _fail("attn_paged: k_cache must be [pages, page_size, kv_heads, dim]")
-    kv_heads = k_cache.shape[2]
-    cshape, sc, tshape, st = _cache(k_cache, v_cache, table, kv_heads, qshape[2], q.dtype, "attn_paged")
+    cshape, sc, tshape, st = _cache(k_cache, v_cache, table, None, qshape[2], q.dtype, "attn_paged")
+    kv_heads = cshape[2]
     batch = tshape[0]
     _ints(lengths, batch, "attn_paged", "lengths")
     return _attn_ragged("attn_paged", q, qshape, sq, k_cache, v_cache, sc[:3], kv_heads, table,
