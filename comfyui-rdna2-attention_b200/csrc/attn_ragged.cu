@@ -27,8 +27,11 @@ extern "C" int b2_attn_ragged(const b2_attn_ragged_args* p, void* stream) {
     if (p->dim != 64 && p->dim != 128) return fail(B2_ERR_UNSUPPORTED, "attn_ragged: head dim %d (64 or 128)", p->dim);
     if (p->dtype != B2_F16 && p->dtype != B2_BF16)
         return fail(B2_ERR_UNSUPPORTED, "attn_ragged: dtype code %d (fp16 or bf16)", p->dtype);
-    if (!(p->scale > 0.f) || p->scale > 3e38f || !(p->softcap >= 0.f) || p->softcap > 3e38f)
-        return fail(B2_ERR_INVALID, "attn_ragged: scale must be positive and softcap not negative, both finite");
+    // Both are multiplied by log2(e), and scores by scale / softcap.
+    if (!(p->scale > 0.f) || p->scale > 2e38f || !(p->softcap >= 0.f) || p->softcap > 2e38f ||
+        (p->softcap > 0.f && p->scale / p->softcap > 2e38f))
+        return fail(B2_ERR_INVALID, "attn_ragged: scale must be positive, softcap not negative, scale, softcap and scale / softcap "
+                                    "at most 2e38");
     if ((int64_t)p->tokens * p->heads > (1 << 30))
         return fail(B2_ERR_UNSUPPORTED, "attn_ragged: %d tokens of %d heads in one call", p->tokens, p->heads);
     if (p->batch == 0 || p->tokens == 0) return B2_OK;

@@ -302,10 +302,27 @@ __device__ __forceinline__ int64_t key_row_offset(const RaggedArgs& a, const Seq
     return (int64_t)page * a.s_page + (int64_t)(key - pi * a.page_size) * a.s_row;
 }
 
-// cap * tanh(x / cap) in the base-2 domain: tanh(y) = 1 - 2 / (1 + 2^(2 y log2 e)). y2 = 2 x log2(e) / cap,
-// cap2 = cap log2(e); saturates to +-cap2 when the power over- or underflows.
+// cap * tanh(s / cap) in the base-2 domain, y = s / cap: tanh(y) = 1 - 2 / (1 + 2^(2 y log2 e)). y2 = 2 y log2(e),
+// cap2 = cap log2(e); saturates to +-cap2 when the power over- or underflows. The difference leaves an error of 3e-7 cap2,
+// small against the score beyond the cap (|y| > 1); inside it tanh_poly keeps the digits.
 __device__ __forceinline__ float capped(float y2, float cap2) {
     return fmaf(-2.f * cap2, rcp_approx(1.f + ex2_approx(y2)), cap2);
+}
+// tanh(y) = y P(y^2), |y| <= 1, P of degree 5 fitted to the smallest relative error (7e-7): y P(y^2) scale on a pair.
+__device__ __forceinline__ uint64_t tanh_poly(uint64_t y, float scale) {
+    const uint64_t u = mul2(y, y);
+    uint64_t p = fma2(splat2(-0.0030670601408928633f * scale), u, splat2(0.016743114218115807f * scale));
+    p = fma2(p, u, splat2(-0.051605671644210815f * scale));
+    p = fma2(p, u, splat2(0.13281433284282684f * scale));
+    p = fma2(p, u, splat2(-0.3332904279232025f * scale));
+    p = fma2(p, u, splat2(0.9999994039535522f * scale));
+    return mul2(y, p);
+}
+// Each of a pair by the form that is accurate for it, so that the relative error stays below 2^-20 whatever the cap is.
+__device__ __forceinline__ uint64_t capped_pair(uint64_t y, float cap2) {
+    const float2 f = upk2(y), p = upk2(tanh_poly(y, cap2));
+    return pk2(fabsf(f.x) <= 1.f ? p.x : capped(f.x * (2.f * RAGGED_LOG2E), cap2),
+               fabsf(f.y) <= 1.f ? p.y : capped(f.y * (2.f * RAGGED_LOG2E), cap2));
 }
 
 template <class T>

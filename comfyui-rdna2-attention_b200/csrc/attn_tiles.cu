@@ -70,17 +70,6 @@ __device__ __forceinline__ void put2(uint32_t (&v)[N], int e, uint64_t x) {
     v[e + 1] = __float_as_uint(f.y);
 }
 
-// tanh(y) = y P(y^2), |y| <= 1, P of degree 5 fitted to the smallest relative error (7e-7): y P(y^2) scale on a pair.
-__device__ __forceinline__ uint64_t tanh_poly(uint64_t y, float scale) {
-    const uint64_t u = mul2(y, y);
-    uint64_t p = fma2(splat2(-0.0030670601408928633f * scale), u, splat2(0.016743114218115807f * scale));
-    p = fma2(p, u, splat2(-0.051605671644210815f * scale));
-    p = fma2(p, u, splat2(0.13281433284282684f * scale));
-    p = fma2(p, u, splat2(-0.3332904279232025f * scale));
-    p = fma2(p, u, splat2(0.9999994039535522f * scale));
-    return mul2(y, p);
-}
-
 // A loading warp's copies in flight: up to three groups, each with the barrier it completes.
 struct Pending {
     uint64_t* bar[3];
@@ -695,7 +684,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         } while (next_list(count, false));
     } else {
         regs_inc<REGS_SOFTMAX>();
-        constexpr bool CAP = MODE & 1, SLOPE = MODE & 2;
+        constexpr bool CAP = MODE & 1, SLOPE = MODE & 2, LARGE = MODE & 4;
         // Softmax of pipeline t = warp / 4.
         const int t = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -795,11 +784,16 @@ __global__ void __launch_bounds__(THREADS, 1)
                                     for (int q = 0; q < 2; ++q)
                                         am[q] = max3(am[q], fabsf(__uint_as_float(w[e + 2 * q])),
                                                      fabsf(__uint_as_float(w[e + 2 * q + 1])));
-                                // Inside the cap by the polynomial, else by exponential and reciprocal.
+                                // All inside the cap: the polynomial. Else exponential and reciprocal, or with a large cap
+                                // each score by the form that is accurate for it.
                                 if (__all_sync(0xffffffffu, fmaxf(am[0], am[1]) * cap_y <= 1.f)) {
 #pragma unroll
                                     for (int e = 0; e < 32; e += 2)
                                         put2(w, e, tanh_poly(mul2(get2(w, e), splat2(cap_y)), cap2));
+                                } else if (LARGE) {
+#pragma unroll
+                                    for (int e = 0; e < 32; e += 2)
+                                        put2(w, e, capped_pair(mul2(get2(w, e), splat2(cap_y)), cap2));
                                 } else {
 #pragma unroll
                                     for (int e = 0; e < 32; ++e)
@@ -961,7 +955,10 @@ int launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap
 int64_t tiles_workspace(int dim) { return ragged_workspace(sm_count(), ROWS, dim); }
 
 int attn_tiles(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t s) {
-    const int mode = (a.softcap > 0.f ? 1 : 0) | (a.slopes ? 2 : 0);
+    // 1: capped scores, 2: bias by distance, 4: a cap beyond 128, where the exponential's form of tanh is off by more than
+    // 1e-4 inside the cap (capped). A variant of its own: the code for it beside the usual caps' made those 2 to 5 % slower
+    // (three packed documents of 700 to 2100 tokens with a cap of 50: 128.5 us against 125.7).
+    const int mode = (a.softcap > 0.f ? 1 : 0) | (a.slopes ? 2 : 0) | (a.softcap > 128.f ? 4 : 0);
     ragged_slots(a, workspace, sm_count(), ROWS, dim);
     // A TMA box is as many rows as divide both a page and a unit; below 8 rows it would cut the swizzle's pattern, and a
     // stride the map cannot hold has none: those caches are gathered by cp.async.
@@ -975,7 +972,9 @@ int attn_tiles(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t 
         case 0: return tma ? launch_tiles<T, D, 0, true>(tq, tk, tv, a, s) : launch_tiles<T, D, 0, false>(tq, tk, tv, a, s); \
         case 1: return tma ? launch_tiles<T, D, 1, true>(tq, tk, tv, a, s) : launch_tiles<T, D, 1, false>(tq, tk, tv, a, s); \
         case 2: return tma ? launch_tiles<T, D, 2, true>(tq, tk, tv, a, s) : launch_tiles<T, D, 2, false>(tq, tk, tv, a, s); \
-        default: return tma ? launch_tiles<T, D, 3, true>(tq, tk, tv, a, s) : launch_tiles<T, D, 3, false>(tq, tk, tv, a, s); \
+        case 3: return tma ? launch_tiles<T, D, 3, true>(tq, tk, tv, a, s) : launch_tiles<T, D, 3, false>(tq, tk, tv, a, s); \
+        case 5: return tma ? launch_tiles<T, D, 5, true>(tq, tk, tv, a, s) : launch_tiles<T, D, 5, false>(tq, tk, tv, a, s); \
+        default: return tma ? launch_tiles<T, D, 7, true>(tq, tk, tv, a, s) : launch_tiles<T, D, 7, false>(tq, tk, tv, a, s); \
     }
     if (dim == 128) {
         if (bf16) {

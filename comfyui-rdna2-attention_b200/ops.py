@@ -817,8 +817,9 @@ def _attn_ragged(name, q, qshape, sq, k, v, sk, kv_heads, table, table_dims, cu_
             _fail(f"{name} slopes must be contiguous fp32 [{heads}]")
         given.append(slopes)
     scale = (0.125 if dim == 64 else 128 ** -0.5) if scale is None else float(scale)
-    if not 0 < scale < 3e38 or not 0 <= softcap < 3e38 or window < 0:
-        _fail(f"{name}: scale {scale} must be positive, softcap {softcap} and window {window} not negative")
+    if not 0 < scale < 2e38 or not 0 <= softcap < 2e38 or window < 0 or (softcap and scale / softcap > 2e38):
+        _fail(f"{name}: scale {scale} must be positive, softcap {softcap} and window {window} not negative (scale, softcap and "
+              f"scale / softcap below 2e38)")
     if out is None:
         out = torch.empty_like(q, memory_format=_contiguous)
         so = out.stride()
