@@ -75,6 +75,7 @@ extern "C" int b2_attn_ragged(const b2_attn_ragged_args* p, void* stream) {
     if (a.table) a.by_page.set(a.page_size);
     a.scale = p->scale;
     a.softcap = p->softcap;
+    a.cap_y = p->softcap > 0.f ? p->scale / p->softcap : 0.f;
     auto kernel = few_rows(p->heads, p->kv_heads, p->dim, p->max_q) ? attn_rows : attn_tiles;
     return kernel(a, p->dim, p->dtype == B2_BF16, p->workspace, (cudaStream_t)stream);
 }

@@ -41,6 +41,7 @@ struct RaggedArgs {
     int batch, tokens, key_rows, heads, kv_heads, group;
     int causal, window;
     float scale, softcap;
+    float cap_y;  // scale / softcap: tanh's argument per unit of q.k
     Divisor by_group, by_page;
     int box_rows;  // attn_tiles.cu: rows of a TMA box of keys
     int q_tma;     // and whether the queries come by TMA

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const 
         const int lo_all = __reduce_max_sync(0xffffffffu, max(lo[0], lo[1]));
         const int hi_all = __reduce_min_sync(0xffffffffu, min(hi[0], hi[1]));
         const float scale2 = a.scale * RAGGED_LOG2E;
-        const float cap2 = a.softcap * RAGGED_LOG2E, cap_y = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+        const float cap2 = a.softcap * RAGGED_LOG2E;
 
         float o[D / 8][4];
 #pragma unroll
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const 
                 for (int e = 0; e < 4; e += 2) {
                     float2 y = make_float2(sc[t][e] * scale2, sc[t][e + 1] * scale2);
                     if (BIAS) {
-                        if (a.softcap > 0.f) y = upk2(capped_pair(mul2(pk2(sc[t][e], sc[t][e + 1]), splat2(cap_y)), cap2));
+                        if (a.softcap > 0.f) y = upk2(capped_pair(mul2(pk2(sc[t][e], sc[t][e + 1]), splat2(a.cap_y)), cap2));
                         const int key = key0 + 8 * t + 2 * (lane & 3);
                         y.x = fmaf(-slope[e >> 1], (float)abs(pos[e >> 1] - key), y.x);
                         y.y = fmaf(-slope[e >> 1], (float)abs(pos[e >> 1] - key - 1), y.y);

@@ -6,6 +6,8 @@ import pytest
 import torch
 
 from ragged_ref import attend64, attend_check
+from test_attn_ragged_gpu import fill
+from test_rope_gpu import paged
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +60,47 @@ def test_large_cap_beside_scores_beyond_it(pkg, dev, dtype, rows, slope, cap):
     want, l64, mass = attend64(q, k, v, softcap=cap, slopes=slopes)
     attend_check(out, want, mass, dtype, m, v.abs().max().item())
     assert ((lse.double() - l64).abs() < 2e-4).all()
+
+
+# ---------------------------------------------------------------- rows beside the live ones
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("opts", [dict(), dict(softcap=20.0), dict(slopes=True), dict(causal=False)])
+@pytest.mark.parametrize("heads,D,page", [(4, 128, 64), (4, 64, 16), (3, 64, 64), (4, 128, 24), (4, 128, 4)])
+def test_a_sequence_does_not_depend_on_its_neighbours(pkg, dev, rows, opts, heads, D, page):
+    """Bit for bit: the first sequence's rows share a tile with rows that hold nothing of its own, and its last page goes on
+    behind its end; neither the next sequence's queries nor what stands there may move as much as a rounding."""
+    counts, ctx = [33, 40, 1500], [600, 90, 5000]  # the third one's work makes the first one's keys one run
+    kc, vc, table, cu, lengths = paged(dev, F16, 1, D, page, counts, ctx, 30)
+    fill(kc, vc, table, lengths, 30)
+    T = sum(counts)
+    q = randn(dev, (T, heads, D), 31, F16, 2.0)
+    opts = dict(opts)
+    if opts.pop("slopes", False):
+        opts["slopes"] = torch.linspace(0.01, 0.3, heads, device=dev)
+    got = []
+    for gain, junk in ((1.0, 0.0), (30.0, 40.0), (0.0, float("nan"))):
+        q2, kc2, vc2 = q.clone(), kc.clone(), vc.clone()
+        q2[33:] *= gain
+        for b, total in enumerate(lengths.tolist()):
+            for c in (kc2, vc2):  # rows behind the end of the last page
+                c[table[b, (total - 1) // page].long(), (total - 1) % page + 1:] = junk
+        lse = torch.empty((T, heads), device=dev)
+        out = pkg.ops.attn_paged(q2, kc2, vc2, table, cu, lengths, lse=lse, max_q=rows, **opts)
+        got.append((out[:33].clone(), lse[:33].clone()))
+    for out, lse in got[1:]:
+        assert torch.equal(out, got[0][0]) and torch.equal(lse, got[0][1])
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_a_packed_document_does_not_depend_on_the_next(pkg, dev, rows):
+    """The same for packed rows: a tile of keys reaches into the next document."""
+    n = [937, 200, 9000]
+    q, k, v = (randn(dev, (sum(n), h, 128), s, BF16, 2.0) for h, s in ((2, 33), (1, 34), (1, 35)))
+    got = []
+    for gain in (1.0, 50.0, float("nan")):
+        q2, k2, v2 = q.clone(), k.clone(), v.clone()
+        for t in (q2, k2, v2):
+            t[937:] *= gain
+        cu = starts(dev, *n)
+        got.append(pkg.ops.attn_packed(q2, k2, v2, cu, cu, max_q=rows)[:937].clone())
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
