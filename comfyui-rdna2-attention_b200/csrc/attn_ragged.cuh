@@ -81,12 +81,16 @@ __device__ __forceinline__ int key_lo(const RaggedArgs& a, const Sequence& s, in
     return a.window ? max(0, s.pos0 + tok - a.window + 1) : 0;
 }
 
+// The first key that any row of row tile rt sees: its first row's.
+template <int ROWS>
+__device__ __forceinline__ int item_from(const RaggedArgs& a, const Sequence& s, int rt) {
+    return key_lo(a, s, a.by_group.of(rt * ROWS));
+}
 // The units [u0, u1) of the keys that any row of row tile rt sees.
 template <int ROWS, int UNIT>
 __device__ __forceinline__ int2 item_units(const RaggedArgs& a, const Sequence& s, int rt) {
-    const int tok0 = a.by_group.of(rt * ROWS);
     const int tok1 = min(s.n - 1, a.by_group.of(rt * ROWS + ROWS - 1));
-    const int hi = key_hi(a, s, tok1), lo = key_lo(a, s, tok0);
+    const int hi = key_hi(a, s, tok1), lo = item_from<ROWS>(a, s, rt);
     if (hi <= lo) return make_int2(0, 1);
     return make_int2(lo / UNIT, (hi + UNIT - 1) / UNIT);
 }
@@ -288,11 +292,12 @@ __device__ __forceinline__ int4 describe(const RaggedArgs& a, const Sequence& s,
     return make_int4(parts | min(ROWS, s.n * a.group - rt * ROWS) << 16, s.q0, kvh, rt * ROWS);
 }
 
-// Element offset of a key row of the sequence in k and v (head 0), or -1: behind the last key, or on a page that does
-// not exist (reported in *status; the row then counts as zeros).
-__device__ __forceinline__ int64_t key_row_offset(const RaggedArgs& a, const Sequence& s, int b, int key,
+// Element offset of a key row of the sequence in k and v (head 0), or -1 for a row that counts as zeros: behind the last
+// key, before the first key `from` that the item sees (a sliding window's old pages may be gone), or on a page that does
+// not exist (reported in *status).
+__device__ __forceinline__ int64_t key_row_offset(const RaggedArgs& a, const Sequence& s, int b, int key, int from,
                                                   unsigned int* status) {
-    if (key >= s.len) return -1;
+    if (key >= s.len || key < from) return -1;
     if (!a.table) return (s.key0 + key) * a.s_row;
     const int pi = a.by_page.of(key);
     const int page = a.table[(int64_t)b * a.table_ld + pi];

@@ -97,8 +97,9 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const 
         // Loads of the run's i-th unit into stage i % STAGES. The lane's row (of 16) is found one unit ahead.
         const T* kh = static_cast<const T*>(a.k) + c.kvh * a.s_head;
         const T* vh = static_cast<const T*>(a.v) + c.kvh * a.s_head;
+        const int from = item_from<ROWS>(a, s, c.rt);
         auto row_of = [&](int i) -> int64_t {
-            return i < units ? key_row_offset(a, s, c.b, (c.unit + i) * UNIT + warp * KEYS + (lane & 15), &g_status) : -1;
+            return i < units ? key_row_offset(a, s, c.b, (c.unit + i) * UNIT + warp * KEYS + (lane & 15), from, &g_status) : -1;
         };
         int64_t next = row_of(0);
         auto load = [&](int i) {

@@ -329,6 +329,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     Sequence s;
                     s.len = it.len;
                     s.key0 = it.key0;
+                    s.pos0 = it.pos0;
+                    const int from = item_from<ROWS>(a, s, it.rt);
                     const int units = it.end - it.unit, first = it.unit, b = it.b;
                     if (tma_warp) {
                         // Lane -> box: `rows` keys of one page, 64 of their columns.
@@ -338,11 +340,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                             const int key = (first + j) * UNIT + bi * rows;
                             if (j >= units || key >= s.len) return make_int2(0, 0);
                             if (!a.table) return make_int2(0, (int)s.key0 + key);
+                            // A box that the window has left behind may have no page any more.
+                            if (key + rows <= from) return make_int2(a.num_pages, 0);  // outside the map: zeros
                             const int pi = a.by_page.of(key);
                             int page = a.table[(int64_t)b * a.table_ld + pi];
                             if (page < 0 || page >= a.num_pages) {
                                 atomicOr(&g_status, B2_DEV_BAD_PAGE);
-                                page = a.num_pages;  // outside the map: zeros
+                                page = a.num_pages;
                             }
                             return make_int2(page, key - pi * a.page_size);
                         };
@@ -442,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                             bool waited = false;
                             for (int blk = 0; blk < 4; ++blk) {
                                 if (job++ % Q_LOADERS != loader) continue;
-                                const int64_t off = key_row_offset(a, s, b, (first + j) * UNIT + 32 * blk + lane, &g_status);
+                                const int64_t off = key_row_offset(a, s, b, (first + j) * UNIT + 32 * blk + lane, from, &g_status);
                                 if (!waited && !wait_free(&empty[st], ((u >> 1) & 1) ^ 1)) return false;
                                 waited = true;
                                 copy_rows(ring + st * C::TILE, blk, base, off);

@@ -880,8 +880,9 @@ def attn_paged(q, k_cache, v_cache, table, cu_q, lengths, scale=None, causal=Tru
     dim^-0.5 unless given): softcap > 0 makes it softcap tanh(s / softcap), slopes (fp32 [heads]) then subtract
     slopes[h] |p - j|. A token that sees no key gets zeros. Rows behind the last sequence are left as they were.
 
-    fp16 or bf16, dim 64 or 128, any group of query heads per KV head, any page size; 16-byte aligned rows. Positions
-    behind a sequence's end and pages it does not use are never read. Keys and values are multiplied a tile at a time with
+    fp16 or bf16, dim 64 or 128, any group of query heads per KV head, any page size; 16-byte aligned rows. What stands
+    behind a sequence's end does not affect results; pages it does not use are not read, nor, with a window, those that lie
+    before the first key that its first new token sees (their table entries may be anything). Keys and values are multiplied a tile at a time with
     zero weights where they are hidden, so a NaN or infinity in v reaches the tokens beside those that see it. ``lse``
     (fp32 [tokens, heads]) receives log sum exp(s). ``max_q``, the new tokens of the longest sequence, chooses the kernel
     (default: the mean). ``workspace`` (b2_attn_ragged_workspace_bytes, allocated when not given) must not be shared by

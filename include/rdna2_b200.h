@@ -319,7 +319,8 @@ int b2_kv_append(const b2_kv_append_args* args, void* stream);
  * and sees key j where (not causal or j <= pos or j < prefix[b]) and (window == 0 or pos - j < window):
  *   s = scale q.k;  s = softcap tanh(s / softcap) if softcap > 0;  s -= slopes[h] |pos - j| if slopes;
  *   out = sum softmax(s) v;  lse = log sum exp(s)
- * A token that sees nothing gets zeros (lse -inf). Keys are pages (table given, lengths int32 [batch]) or packed rows
+ * A token that sees nothing gets zeros (lse -inf). Pages before the first key that a sequence's first new token sees need
+ * not exist. Keys are pages (table given, lengths int32 [batch]) or packed rows
  * (table null, lengths = cu_k int32 [batch + 1], k and v [key_rows, kv_heads, dim] with strides s_row, s_head).
  * dim 64 or 128, fp16 or bf16, heads a multiple of kv_heads; every pointer 16-byte aligned and every stride a multiple
  * of 8 elements; scale positive, softcap not negative, both and scale / softcap at most 2e38. max_q, an upper bound of the new tokens per sequence, chooses the kernel and nothing else. workspace:

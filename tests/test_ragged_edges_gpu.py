@@ -5,8 +5,8 @@ import math
 import pytest
 import torch
 
-from ragged_ref import attend64, attend_check
-from test_attn_ragged_gpu import fill
+from ragged_ref import attend64, attend_check, pages_of
+from test_attn_ragged_gpu import fill, verify
 from test_rope_gpu import paged
 
 pytestmark = pytest.mark.gpu
@@ -104,3 +104,32 @@ def test_a_packed_document_does_not_depend_on_the_next(pkg, dev, rows):
         cu = starts(dev, *n)
         got.append(pkg.ops.attn_packed(q2, k2, v2, cu, cu, max_q=rows)[:937].clone())
     assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+# ---------------------------------------------------------------- pages before a window
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("gone", ["no page", "outside", "nan"])
+@pytest.mark.parametrize("opts", [dict(window=70), dict(window=300, softcap=20.0), dict(window=33, causal=False, slopes=True)])
+@pytest.mark.parametrize("page", [1, 8, 16, 24, 64])
+def test_pages_before_the_window_are_not_needed(pkg, dev, dtype, rows, gone, opts, page):
+    """A sliding window frees a sequence's old pages: entries without a page, or with one that holds another's values."""
+    counts, ctx, H, Hk, D = [1, 40, 150], [700, 330, 900], 4, 2, 64
+    kc, vc, table, cu, lengths = paged(dev, dtype, Hk, D, page, counts, ctx, 50)
+    fill(kc, vc, table, lengths, 50)
+    opts, total = dict(opts), lengths.tolist()
+    slopes = torch.linspace(0.01, 0.3, H, device=dev) if opts.pop("slopes", False) else None
+    ks = [pages_of(kc, table, b, t).clone() for b, t in enumerate(total)]
+    vs = [pages_of(vc, table, b, t).clone() for b, t in enumerate(total)]
+    for b, (n, c) in enumerate(zip(counts, ctx)):
+        old = max(0, c - opts["window"] + 1) // page  # pages that lie before the first new token's window
+        if gone == "nan":
+            for cache in (kc, vc):
+                cache[table[b, :old].long()] = float("nan")
+        else:
+            table[b, :old] = -1 if gone == "no page" else kc.shape[0]
+    q = randn(dev, (sum(counts), H, D), 51, dtype)
+    lse = torch.empty((sum(counts), H), device=dev)
+    out = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, slopes=slopes, lse=lse, max_q=rows, **opts)
+    assert pkg._lib.device_status() == 0
+    verify(out, lse, q, counts, lambda b: ks[b], lambda b: vs[b], opts, None, dtype, slopes)
