@@ -13,9 +13,13 @@ bool few_rows(int heads, int kv_heads, int dim, int max_q) {
 }
 }  // namespace
 
+// The larger of the two kernels' needs, whatever max_q is: the call cannot tell how large its buffer is, and one that was
+// sized for single tokens may be handed to a chunk.
 extern "C" int64_t b2_attn_ragged_workspace_bytes(int heads, int kv_heads, int dim, int max_q) {
+    (void)max_q;
     if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || (dim != 64 && dim != 128)) return 0;
-    return few_rows(heads, kv_heads, dim, max_q) ? rows_workspace(dim) : tiles_workspace(dim);
+    const int64_t rows = rows_workspace(dim), tiles = tiles_workspace(dim);
+    return rows > tiles ? rows : tiles;
 }
 
 extern "C" int b2_attn_ragged(const b2_attn_ragged_args* p, void* stream) {

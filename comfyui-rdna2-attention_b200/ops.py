@@ -838,7 +838,7 @@ def _attn_ragged(name, q, qshape, sq, k, v, sk, kv_heads, table, table_dims, cu_
         given.append(workspace)
     max_q = -(-tokens // max(batch, 1)) if max_q is None else min(max(int(max_q), 0), 1 << 30)
     device = _one_device(q, k, v, cu_q, lengths, *given)
-    nbytes = _ragged_workspace(device, heads, kv_heads, dim, max_q)
+    nbytes = _ragged_workspace(device, dim)
     if workspace is None:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < nbytes:
@@ -855,20 +855,19 @@ def _attn_ragged(name, q, qshape, sq, k, v, sk, kv_heads, table, table_dims, cu_
     return out
 
 
-_workspace_sizes = {}  # (device, heads, kv heads, dim, max_q) -> bytes: the sizes depend on nothing else
+_workspace_sizes = {}  # (device, dim) -> bytes: the sizes depend on nothing else
 
 
-def _ragged_workspace(*key):
-    nbytes = _workspace_sizes.get(key)
+def _ragged_workspace(device, dim):
+    nbytes = _workspace_sizes.get((device, dim))
     if nbytes is None:
-        if len(_workspace_sizes) >= 4096:
-            _workspace_sizes.clear()
-        if key[0] == torch._C._cuda_getDevice():
-            nbytes = _lib.load().b2_attn_ragged_workspace_bytes(*key[1:])
+        query = _lib.load().b2_attn_ragged_workspace_bytes
+        if device == torch._C._cuda_getDevice():
+            nbytes = query(1, 1, dim, 1)
         else:
-            with torch.cuda.device(key[0]):
-                nbytes = _lib.load().b2_attn_ragged_workspace_bytes(*key[1:])
-        _workspace_sizes[key] = nbytes
+            with torch.cuda.device(device):
+                nbytes = query(1, 1, dim, 1)
+        _workspace_sizes[device, dim] = nbytes
     return nbytes
 
 

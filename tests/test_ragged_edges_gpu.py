@@ -133,3 +133,18 @@ def test_pages_before_the_window_are_not_needed(pkg, dev, dtype, rows, gone, opt
     out = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, slopes=slopes, lse=lse, max_q=rows, **opts)
     assert pkg._lib.device_status() == 0
     verify(out, lse, q, counts, lambda b: ks[b], lambda b: vs[b], opts, None, dtype, slopes)
+
+
+# ---------------------------------------------------------------- workspace
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_workspace_sized_for_tokens_holds_a_chunk(pkg, dev, D):
+    n = pkg._lib.load().b2_attn_ragged_workspace_bytes(4, 1, D, 1)
+    buf = torch.full((n + (1 << 16),), 85, dtype=torch.uint8, device=dev)
+    counts, ctx = [1000, 3, 600], [5000, 700, 20000]
+    kc, vc, table, cu, lengths = paged(dev, F16, 1, D, 16, counts, ctx, 60)
+    fill(kc, vc, table, lengths, 60)
+    q = randn(dev, (sum(counts), 4, D), 61, F16)
+    for rows in ROWS:
+        want = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, max_q=rows)
+        got = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, max_q=rows, workspace=buf[:n])
+        assert torch.equal(got, want) and (buf[n:] == 85).all()

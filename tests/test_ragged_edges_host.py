@@ -25,3 +25,11 @@ def test_factors_at_the_ends_are_taken(pkg, calls):
     for kw in (dict(softcap=1.9e38), dict(softcap=1e-30), dict(scale=1e-30)):
         pkg.ops.attn_paged(**attn(**kw))
     assert len(calls) == 3
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_workspace_serves_every_call_of_a_dim(pkg, dim):
+    """The argument block does not say how large the workspace is: a buffer sized for tokens must hold a chunk's parts too."""
+    size = pkg._lib.load().b2_attn_ragged_workspace_bytes
+    assert len({size(h, k, dim, n) for h, k in ((8, 2), (32, 8), (7, 1), (5, 5)) for n in (0, 1, 4, 17, 1000, 1 << 30)}) == 1
+    assert size(8, 2, dim, 1) > 0 and size(8, 3, dim, 1) == 0 and size(8, 2, 96, 1) == 0
