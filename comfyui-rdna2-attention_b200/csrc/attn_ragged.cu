@@ -8,6 +8,10 @@ namespace {
 // starts sooner and wastes less on few rows. Measured in us, 16-row kernel / 256-row kernel:
 //   dim 128, 24 x 8000 keys: 16 rows 102 / 114, 20 rows 150 / 115;  4 x 16000 keys: 16 rows 51 / 57, 20 rows 83 / 57
 //   dim 64,  32 x 2000 keys: 16 rows 27 / 47, 32 rows 39 / 47, 36 rows 56 / 48
+// One kernel takes the whole batch, so sequences of unlike lengths lose on either side (dim 128):
+//   64 sequences of two tokens over 4000 keys, a row each 166 / 246, four rows each 170 / 247
+//   one of 1000 tokens over 4000 keys beside 99 single tokens over 3000, a row each: 231 / 330; over 61 000 keys: 1851 / 555
+//   one of 500 tokens over 2500 keys beside 200 single tokens over 2000, four rows each: 303 / 440
 bool few_rows(int heads, int kv_heads, int dim, int max_q) {
     return (int64_t)max_q * (heads / kv_heads) <= (dim == 64 ? 32 : 16);
 }

@@ -881,10 +881,12 @@ def attn_paged(q, k_cache, v_cache, table, cu_q, lengths, scale=None, causal=Tru
 
     fp16 or bf16, dim 64 or 128, any group of query heads per KV head, any page size; 16-byte aligned rows. What stands
     behind a sequence's end does not affect results; pages it does not use are not read, nor, with a window, those that lie
-    before the first key that its first new token sees (their table entries may be anything). Keys and values are multiplied a tile at a time with
-    zero weights where they are hidden, so a NaN or infinity in v reaches the tokens beside those that see it. ``lse``
-    (fp32 [tokens, heads]) receives log sum exp(s). ``max_q``, the new tokens of the longest sequence, chooses the kernel
-    (default: the mean). ``workspace`` (b2_attn_ragged_workspace_bytes, allocated when not given) must not be shared by
+    before the first key that its first new token sees (their table entries may be anything). Keys and values are multiplied
+    a tile at a time with zero weights where they are hidden, so a NaN or infinity in v reaches the tokens beside those that
+    see it. ``lse`` (fp32 [tokens, heads]) receives log sum exp(s). ``max_q``, the new tokens of the longest sequence, chooses
+    the kernel and nothing else; not given, the mean stands for it, which suits sequences of like lengths: give it where one
+    is far longer than the others (a long prompt among single tokens can take three times as long without it).
+    ``workspace`` (b2_attn_ragged_workspace_bytes, allocated when not given) must not be shared by
     calls that overlap on the GPU."""
     qshape, sq = _packed(q, "attn_paged q")
     cshape, sc, tshape, st = _cache(k_cache, v_cache, table, None, qshape[2], q.dtype, "attn_paged")

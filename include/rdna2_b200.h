@@ -323,9 +323,10 @@ int b2_kv_append(const b2_kv_append_args* args, void* stream);
  * not exist. Keys are pages (table given, lengths int32 [batch]) or packed rows
  * (table null, lengths = cu_k int32 [batch + 1], k and v [key_rows, kv_heads, dim] with strides s_row, s_head).
  * dim 64 or 128, fp16 or bf16, heads a multiple of kv_heads; every pointer 16-byte aligned and every stride a multiple
- * of 8 elements; scale positive, softcap not negative, both and scale / softcap at most 2e38. max_q, an upper bound of the
- * new tokens per sequence, chooses the kernel and nothing else. workspace: b2_attn_ragged_workspace_bytes bytes (for the
- * call's dim on the call's device; the same for every max_q and batch), not shared by calls that overlap on the GPU. */
+ * of 8 elements; scale positive, softcap not negative, both and scale / softcap at most 2e38. max_q, the new tokens of the
+ * longest sequence as far as it is known, chooses the kernel and nothing else. workspace: b2_attn_ragged_workspace_bytes
+ * bytes (for the call's dim on the call's device; the same for every max_q and batch), not shared by calls that overlap on
+ * the GPU. */
 typedef struct b2_attn_ragged_args {
     const void* q;
     int64_t sqt, sqh;
