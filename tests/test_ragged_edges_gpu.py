@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from ragged_ref import attend64, attend_check, pages_of
+from ragged_ref import HALF_STEP, attend64, attend_check, check, pages_of, rope64, rope_bound
 from test_attn_ragged_gpu import fill, verify
 from test_rope_gpu import paged
 
@@ -148,3 +148,132 @@ def test_a_workspace_sized_for_tokens_holds_a_chunk(pkg, dev, D):
         want = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, max_q=rows)
         got = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, max_q=rows, workspace=buf[:n])
         assert torch.equal(got, want) and (buf[n:] == 85).all()
+
+
+# ---------------------------------------------------------------- bias of far keys
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("cap", [0.0, 9.0])
+@pytest.mark.parametrize("slope", [0.37, 0.0507, -0.2113])
+def test_bias_where_every_key_is_far(pkg, dev, dtype, rows, cap, slope):
+    """More queries than keys (the first query is 20000 positions before the keys' middle) and a bias that grows with the distance:
+    all weights are differences of large biases. A score of magnitude B in the base-2 exponent, formed in fp32 from
+    product and sum, is off by 2 * 2^-24 B, a weight by ln 2 times that, and the sum by as much."""
+    n, m, H, D = 20000, 96, 2, 128
+    q, k, v = randn(dev, (n, H, D), 40, dtype), randn(dev, (m, 1, D), 41, dtype), randn(dev, (m, 1, D), 42, dtype)
+    slopes = torch.tensor([slope, slope / 3], device=dev)
+    lse = torch.empty((n, H), device=dev)
+    out = pkg.ops.attn_packed(q, k, v, starts(dev, n), starts(dev, m), causal=False, softcap=cap, slopes=slopes, lse=lse, max_q=rows)
+    r = torch.arange(0, n, 97, device=dev)
+    dist = (r[:, None] + (m - n) - torch.arange(m, device=dev)[None, :]).abs().double()
+    for h in range(H):
+        s = q[r, h].double() @ k[:, 0].double().t() * D ** -0.5
+        if cap:
+            s = cap * torch.tanh(s / cap)
+        s = s - slopes[h].double() * dist
+        w = torch.softmax(s, 1)
+        want, mass = w @ v[:, 0].double(), w @ v[:, 0].double().abs()
+        B = s.abs().amax(1, keepdim=True) / math.log(2)
+        extra = (HALF_STEP[dtype] + 4e-4 + 2 * math.log(2) * 2.0 ** -23 * B) * mass
+        if dtype == F16:
+            extra = extra + m * 2.0 ** -25 * v.abs().max().item()
+        check(out[r, h], want, extra, dtype)
+        assert ((lse[r, h].double() - torch.logsumexp(s, 1)).abs() < 2e-4 + 2.0 ** -22 * B[:, 0]).all()
+
+
+# ---------------------------------------------------------------- paths that take a special shape
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D,page,opts", [(64, 16, {}), (128, 16, dict(softcap=10.0)), (64, 3, {}), (128, 64, dict(window=20))])
+def test_more_items_than_a_list_holds(pkg, dev, dtype, D, page, opts):
+    """1700 short sequences of 8 KV heads are about 70 items per CTA of the 256-row kernel, which describes 48 at a time; some of
+    several units among them. Compared with one padded 64-bit computation."""
+    B, Hk, G = 1700, 8, 2
+    counts = [(7 * b) % 4 for b in range(B)]
+    ctx = [(37 * b) % 60 + (300 if b % 50 == 0 else 0) for b in range(B)]
+    kc, vc, table, cu, lengths = paged(dev, dtype, Hk, D, page, counts, ctx, 70)
+    m = max(n + c for n, c in zip(counts, ctx))
+    j = torch.arange(m, device=dev)[None, :]
+    there = j < lengths[:, None]
+    at = table[:, :-(-m // page)].long().repeat_interleave(page, 1)[:, :m].masked_fill(~there, 0)
+    k, v = (randn(dev, (B, m, Hk, D), s, dtype) for s in (71, 72))
+    row = (j % page).expand(B, m)
+    for cache, x in ((kc, k), (vc, v)):
+        cache[at[there], row[there]] = x[there]
+    seq = torch.repeat_interleave(torch.arange(B, device=dev), cu.diff().long())
+    pos = torch.arange(len(seq), device=dev) - cu[seq + 1].long() + lengths[seq].long()
+    q = randn(dev, (len(seq), Hk * G, D), 73, dtype)
+    lse = torch.empty((len(seq), Hk * G), device=dev)
+    out = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, lse=lse, max_q=1000, **opts)
+    assert pkg._lib.device_status() == 0
+    vis = (j <= pos[:, None]) & (pos[:, None] - j < opts.get("window", 1 << 30))
+    vmax = v.abs().max().item()
+    for h in range(Hk * G):
+        s = torch.einsum("td,tmd->tm", q[:, h].double(), k[seq, :, h // G].double()) * D ** -0.5
+        if "softcap" in opts:
+            s = opts["softcap"] * torch.tanh(s / opts["softcap"])
+        s = s.masked_fill(~vis, -math.inf)
+        w, vv = torch.softmax(s, 1), v[seq, :, h // G].double()
+        attend_check(out[:, h], torch.einsum("tm,tmd->td", w, vv), torch.einsum("tm,tmd->td", w, vv.abs()), dtype, m, vmax)
+        assert ((lse[:, h].double() - torch.logsumexp(s, 1)).abs() < 2e-4).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("page", [16, 24, 128])
+@pytest.mark.parametrize("H,Hk,D", [(6, 2, 64), (12, 4, 128), (5, 1, 64)])
+@pytest.mark.parametrize("opts", [dict(), dict(softcap=5.0), dict(slopes=True, window=90), dict(causal=False)])
+def test_groups_that_no_box_of_queries_holds(pkg, dev, dtype, page, H, Hk, D, opts):
+    """Three or five heads per KV head do not divide a tile's 128 rows: keys come by TMA, queries row by row."""
+    counts, ctx = [100, 2, 43], [50, 300, 0]
+    kc, vc, table, cu, lengths = paged(dev, dtype, Hk, D, page, counts, ctx, 80)
+    fill(kc, vc, table, lengths, 80)
+    q = randn(dev, (sum(counts), H, D), 81, dtype, 2.0)
+    opts, total = dict(opts), lengths.tolist()
+    slopes = torch.linspace(0.01, 0.3, H, device=dev) if opts.pop("slopes", False) else None
+    lse = torch.empty((sum(counts), H), device=dev)
+    out = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, slopes=slopes, lse=lse, max_q=100, **opts)
+    verify(out, lse, q, counts, lambda b: pages_of(kc, table, b, total[b]), lambda b: pages_of(vc, table, b, total[b]),
+           opts, None, dtype, slopes)
+
+
+@pytest.mark.parametrize("H,D", [(32, 64), (64, 128), (128, 128), (160, 64), (300, 64)])
+@pytest.mark.parametrize("opts", [dict(), dict(softcap=5.0, slopes=True, window=90)])
+def test_many_heads_on_one_kv_head(pkg, dev, H, D, opts):
+    """A token of 128 heads is a tile by itself; one of 160 or 300 begins and ends inside tiles."""
+    counts, ctx = [3, 1, 2], [140, 300, 0]
+    kc, vc, table, cu, lengths = paged(dev, BF16, 1, D, 16, counts, ctx, 85)
+    fill(kc, vc, table, lengths, 85)
+    q = randn(dev, (sum(counts), H, D), 86, BF16, 2.0)
+    opts, total = dict(opts), lengths.tolist()
+    slopes = torch.linspace(0.01, 0.3, H, device=dev) if opts.pop("slopes", False) else None
+    lse = torch.empty((sum(counts), H), device=dev)
+    out = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths, slopes=slopes, lse=lse, **opts)
+    verify(out, lse, q, counts, lambda b: pages_of(kc, table, b, total[b]), lambda b: pages_of(vc, table, b, total[b]),
+           opts, None, BF16, slopes)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, torch.float32])
+@pytest.mark.parametrize("tokens", [592, 593, 594, 595, 1777])
+@pytest.mark.parametrize("dim,rot,interleaved", [(64, 64, False), (96, 32, True), (10, 6, False)])
+def test_four_tokens_per_cta_and_the_rest(pkg, dev, dtype, tokens, dim, rot, interleaved):
+    """Many tokens are rotated four to a CTA: counts that leave one, two or three in the last one, each token with its own
+    angles and its own place in the cache; heads of 10 values go value by value."""
+    inv, _ = pkg.ops.rope_frequencies(rot, device=dev)
+    x = randn(dev, (tokens, 3, dim), 90, dtype)
+    pos = torch.randint(0, 1 << 20, (tokens,), generator=torch.Generator().manual_seed(tokens)).to(dev)
+    want = rope64(x, pos, inv, interleaved)
+    check(pkg.ops.rope(x, pos, inv, interleaved=interleaved), want, rope_bound(x, want, inv, interleaved), dtype)
+    counts = [tokens - 5 - tokens // 3 - 2, 5, 0, tokens // 3]  # two rows behind the last sequence
+    ctx = [30, 0, 9, 100]
+    kc, vc, table, cu, lengths = paged(dev, dtype, 1, dim, 16, counts, ctx, 91)
+    q, k, v = x[:, :1], x[:, 1:2], x[:, 2:]
+    q_out = torch.full((tokens, 1, dim), 7.0, dtype=dtype, device=dev)
+    pkg.ops.kv_append(k, v, kc, vc, table, cu, lengths, inv_freq=inv, q=q, q_out=q_out, interleaved=interleaved)
+    assert (q_out[-2:] == 7.0).all() and pkg._lib.device_status() == 0
+    at = 0
+    for b, (n, c) in enumerate(zip(counts, ctx)):
+        r, here = slice(at, at + n), torch.arange(c, c + n, device=dev)
+        at += n
+        for got, src in ((q_out[r], q[r]), (pages_of(kc, table, b, c + n)[c:], k[r])):
+            want = rope64(src, here, inv, interleaved)
+            check(got, want, rope_bound(src, want, inv, interleaved), dtype)
+        assert torch.equal(pages_of(vc, table, b, c + n)[c:], v[r])
