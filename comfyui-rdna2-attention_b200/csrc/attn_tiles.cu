@@ -13,8 +13,8 @@
 //   warps 8..10       instead, the rows gathered by cp.async where no box fits (odd page sizes, odd groups for queries)
 //   warp 11           issues the products
 //   warps 12..15      epilogue: O out of TMEM while the softmax warps are at the next item
-// Rows of V behind a sequence's last key are zero in shared memory, so nothing stale is multiplied, and rows of an item
-// behind its last one have no say in its warps' votes: a sequence's bits do not depend on what lies beside it.
+// Rows of V behind a sequence's last key are zero in shared memory, so nothing stale is multiplied; rows of an item behind
+// its last one and keys behind the end have no say in the warps' votes: a sequence's bits do not depend on what lies beside it.
 //
 // Measured (32 query heads over 8 kv heads of 128, bf16): 2048 tokens over 65 000 keys 1.94 ms, 1106 TFLOP/s, 0.67 of the
 // measured bf16 rate (2.3 ms where the power cap holds the clock near 1.4 GHz); 12 packed documents of 50 to 4000 tokens
@@ -218,7 +218,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t* ml_full = bars + 20; // [2]
     uint64_t* drain = bars + 22;
     uint64_t* v_tail = bars + 23;
-    uint64_t* k_tail = bars + 26;  // behind tmem_slot, abort_flag and list_len
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* list_len = abort_flag + 1;  // items in the list; negative: the last list
@@ -244,7 +243,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(&ml_full[i], 4);
         }
         mbar_init(v_tail, 1);
-        mbar_init(k_tail, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -297,8 +295,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             constexpr uint32_t Q_LOADERS = TMA ? LOADERS - 1 : LOADERS;
             const uint32_t loader = warp - LOAD_WARP - (TMA ? 1 : 0);
             const bool tma_warp = TMA && warp == LOAD_WARP;
-            uint32_t v_tails = 0, k_tails = 0, k_issued = 0, v_issued = 0, q_issued = 0;
-            int k_open = -1;  // keys of a last unit of keys that is on its way to k_tail
+            uint32_t tails = 0, k_issued = 0, v_issued = 0, q_issued = 0;
             uint32_t items_done = 0, units_done = 0, job = 0;
             int count;
             do {
@@ -371,42 +368,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                                             it.kvh, at.x);
                             return max(keys, 0);
                         };
-                        // Rows behind the last key hold whatever the page or the stage held before. V's product takes them times
-                        // zero, so they must be finite; a capped score of theirs would have a say in the choice of the cap's
-                        // form for the chunk, so K's are cleared too, once the next copies are on their way.
-                        auto clear_tail = [&](unsigned char* ring, uint64_t* full, int j, int keys, uint64_t* tail,
-                                              uint32_t n) -> bool {
-                            const int st = (units_done + j) & 1;
-                            const bool there = mbar_wait(tail, n & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_PRODUCER);
-                            if (!there && !mbar_wait_drain(tail, n & 1, 100000000ull)) atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
-                            for (int c = keys * 8 + lane; c < UNIT * 8; c += 32)
-#pragma unroll
-                                for (int h = 0; h < D / 64; ++h)
-                                    *reinterpret_cast<uint4*>(ring + st * C::TILE + h * (128 * 128) + c * 16) = make_uint4(0, 0, 0, 0);
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&full[st]);
-                            return there;
-                        };
-                        auto is_tail = [&](int j) { return (first + j + 1) * UNIT > s.len; };
-                        auto load_k = [&](int j, int2 where) -> bool {
-                            const bool tail = (MODE & 1) && is_tail(j);
-                            const int keys = load_unit(&tmK, sK, k_full, k_empty, j, where, tail ? k_tail : nullptr);
-                            if (tail)
-                                k_open = keys;
-                            else if (keys >= 0)
-                                ++k_issued;
-                            return keys >= 0;
-                        };
-                        auto finish_k = [&](int j) -> bool {
-                            if (!(MODE & 1) || k_open < 0) return true;
-                            const bool there = clear_tail(sK, k_full, j, k_open, k_tail, k_tails++);
-                            k_open = -1;
-                            if (there) ++k_issued;
-                            return there;
-                        };
                         int2 at = place(0);
-                        ok = load_k(0, at);
+                        ok = load_unit(&tmK, sK, k_full, k_empty, 0, at, nullptr) >= 0;
+                        if (ok) ++k_issued;
                         if (ok && a.q_tma) {
                             // 128 rows are 128 / group tokens of group heads. A second tile without rows is not loaded.
                             ok = wait_free(q_empty, (items_done & 1) ^ 1);
@@ -422,19 +386,33 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 ++q_issued;
                             }
                         }
-                        ok = ok && finish_k(0);
                         for (int j = 0; j < units && ok; ++j) {
                             const int2 next = place(j + 1);
                             if (j + 1 < units) {
-                                ok = load_k(j + 1, next);
+                                ok = load_unit(&tmK, sK, k_full, k_empty, j + 1, next, nullptr) >= 0;
                                 if (!ok) break;
+                                ++k_issued;
                             }
-                            const bool tail = is_tail(j);
+                            const bool tail = (first + j + 1) * UNIT > s.len;
                             const int keys = load_unit(&tmV, sV, v_full, v_empty, j, at, tail ? v_tail : nullptr);
                             ok = keys >= 0;
-                            if (ok && tail) ok = clear_tail(sV, v_full, j, keys, v_tail, v_tails++);
+                            if (ok && tail) {
+                                // Rows behind the last key hold whatever the page or the stage held before; the product
+                                // takes them times zero, so they must be finite.
+                                ok = mbar_wait(v_tail, tails & 1, abort_flag, &g_status, B2_DEV_TIMEOUT_PRODUCER);
+                                if (!ok && !mbar_wait_drain(v_tail, tails & 1, 100000000ull))
+                                    atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
+                                ++tails;
+                                unsigned char* tile = sV + ((units_done + j) & 1) * C::TILE;
+                                for (int c = keys * 8 + lane; c < UNIT * 8; c += 32)
+#pragma unroll
+                                    for (int h = 0; h < D / 64; ++h)
+                                        *reinterpret_cast<uint4*>(tile + h * (128 * 128) + c * 16) = make_uint4(0, 0, 0, 0);
+                                fence_proxy_async_smem();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(&v_full[(units_done + j) & 1]);
+                            }
                             if (ok) ++v_issued;
-                            ok = ok && finish_k(j + 1);
                             at = next;
                         }
                     } else if (!TMA || !a.q_tma) {
@@ -483,7 +461,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                     // Given up: the copies in flight must land before the CTA ends.
                     if (q_issued && !mbar_wait_drain(q_full, (q_issued - 1) & 1, 100000000ull))
                         atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
-                    if (k_open >= 0 && !mbar_wait_drain(k_tail, k_tails & 1, 100000000ull)) atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
                     for (uint32_t n = 1; n <= 2; ++n) {
                         if (k_issued >= n && !mbar_wait_drain(&k_full[(k_issued - n) & 1], ((k_issued - n) >> 1) & 1, 100000000ull))
                             atomicOr(&g_status, B2_DEV_TIMEOUT_DRAIN);
@@ -718,7 +695,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lane_base + t * UNIT, tO = tmem + lane_base + 256 + t * D;
         const float scale2 = a.scale * RAGGED_LOG2E;
-        const float cap2 = a.softcap * RAGGED_LOG2E, cap_in = 2.f * RAGGED_LOG2E * a.cap_y;
+        const float cap2 = a.softcap * RAGGED_LOG2E, cap_in = CAP ? 2.f * scale2 / a.softcap : 0.f;
+        const float cap_y = CAP ? a.scale / a.softcap : 0.f;  // tanh's argument per unit of raw score
         uint32_t ucount = 0, icount = 0;
         int count;
         do {
@@ -802,11 +780,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                         // the instruction cache next to the scheduler, and a unit took twice as long.
                         float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                         const int2 seen_keys = part ? row_keys() : make_int2(0, 0x7fffffff);
+                        const int there = it.len - key0;  // keys of the unit; what stands behind them is masked below
 #pragma unroll 1
                         for (int c = 0; c < 128; c += 32) {
                             uint32_t w[32];
                             tmem_ld32_wait(tS + c, w);
-                            if (CAP) {
+                            if (CAP && c < there) {
                                 float am[2] = {0.f, 0.f};
 #pragma unroll
                                 for (int e = 0; e < 32; e += 4)
@@ -815,15 +794,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                                         am[q] = max3(am[q], fabsf(__uint_as_float(w[e + 2 * q])),
                                                      fabsf(__uint_as_float(w[e + 2 * q + 1])));
                                 // All inside the cap: the polynomial. Else exponential and reciprocal, or with a large cap
-                                // each score by the form that is accurate for it.
-                                if (__all_sync(0xffffffffu, fmaxf(am[0], am[1]) <= inside)) {
+                                // each score by the form that is accurate for it. The choice moves a rounding, so where the end
+                                // falls inside the chunk it is not the scores' (K cleared behind the end instead: 24 drafts over
+                                // up to 9000 keys 3 % slower, as the loads wait for the last unit).
+                                if (__all_sync(0xffffffffu, fmaxf(am[0], am[1]) <= (c + 32 <= there ? inside : -1.f))) {
 #pragma unroll
                                     for (int e = 0; e < 32; e += 2)
-                                        put2(w, e, tanh_poly(mul2(get2(w, e), splat2(a.cap_y)), cap2));
+                                        put2(w, e, tanh_poly(mul2(get2(w, e), splat2(cap_y)), cap2));
                                 } else if (LARGE) {
 #pragma unroll
                                     for (int e = 0; e < 32; e += 2)
-                                        put2(w, e, capped_pair(mul2(get2(w, e), splat2(a.cap_y)), cap2));
+                                        put2(w, e, capped_pair(mul2(get2(w, e), splat2(cap_y)), cap2));
                                 } else {
 #pragma unroll
                                     for (int e = 0; e < 32; ++e)
