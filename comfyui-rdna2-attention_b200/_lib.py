@@ -61,7 +61,6 @@ SIGNATURES = {
     "b2_attn_ragged": (I, [P, P]),
 }
 
-
 _lib = None
 
 

@@ -308,6 +308,12 @@ __device__ __forceinline__ int64_t key_row_offset(const RaggedArgs& a, const Seq
     return (int64_t)page * a.s_page + (int64_t)(key - pi * a.page_size) * a.s_row;
 }
 
+// 16 bytes into shared memory, zeros where !ok (nothing is read then).
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+    const int n = ok ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
 // cap * tanh(s / cap) in the base-2 domain, y = s / cap: tanh(y) = 1 - 2 / (1 + 2^(2 y log2 e)). y2 = 2 y log2(e),
 // cap2 = cap log2(e); saturates to +-cap2 when the power over- or underflows. The difference leaves an error of 3e-7 cap2,
 // small against the score beyond the cap (|y| > 1); inside it tanh_poly keeps the digits.
@@ -418,7 +424,6 @@ __global__ void __launch_bounds__(512) merge_kernel(const RaggedArgs a) {
         *reinterpret_cast<uint32_t*>(dst) = u[0];
     if (a.lse && lane == 0) a.lse[(int64_t)tok * a.heads + head] = log_sum(M, L);
 }
-  // two 16-bit values of T from fp32, rounded to nearest even
 
 // ---------------------------------------------------------------- host
 // Workspace of a launch of `ctas` CTAs: two slots each of ROWS rows of O and (m, l), and the descriptors.

@@ -1,8 +1,8 @@
 // Ragged attention for few rows per kv head (tokens being decoded): 16 rows per item on mma.sync m16n8k16.
 //
 // With r = tokens x G rows per kv head the work is 4 D r flops per key and kv head against 4 D bytes of keys and
-// values: at 16 rows that is 4 flops per byte, so HBM bounds it and the legacy tensor path (16-row tiles, operands in
-// registers) is enough; a tcgen05 tile would be 128 rows of which at most 16 hold anything.
+// values, r flops per byte: 16 at 16 rows, where the tensor cores bound from 252 on, so HBM bounds it and the legacy tensor
+// path (16-row tiles, operands in registers) is enough; a tcgen05 tile would be 128 rows of which at most 16 hold anything.
 //
 // A CTA is four warps, each its own pipeline: warp w takes keys [64 u + 16 w, + 16) of every unit u of the run, loads
 // their K and V rows with cp.async (16 bytes a lane, rows gathered through the page table; rows behind the last key
@@ -31,10 +31,6 @@ struct Cfg {
     static constexpr int CTAS = D == 128 ? 2 : 3;             // per SM
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-    const int n = ok ? 16 : 0;  // 0 source bytes: 16 zero bytes are written
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {

@@ -1,7 +1,8 @@
 // Ragged attention for many rows per kv head (chunks of prompts, packed documents): 256 rows per item on tcgen05.
 //
-// With 256 rows an item does 1024 D flops per key against 4 D bytes of keys and values, well above the 250 flops per
-// byte where the tensor cores become the bound. Two pipelines A and B work in ping-pong: while the softmax warps of one
+// With 256 rows an item does 1024 D flops per key against 4 D bytes of keys and values, 256 per byte: just where the tensor
+// cores become the bound (1654 TFLOP/s over 6.55 TB/s are 252), and well inside it as the other row tiles and query heads
+// find the same keys in L2. Two pipelines A and B work in ping-pong: while the softmax warps of one
 // work on its scores, the tensor core works for the other (S, P and O in TMEM, P written back over the consumed scores
 // as the A operand of the second product). An item of more than 128 rows puts its first 128 on A and the others on B,
 // each over the units that its own rows see. An item of up to 128 rows (short chunks, drafts being checked), which HBM
@@ -14,11 +15,11 @@
 //   warp 11           issues the products
 //   warps 12..15      epilogue: O out of TMEM while the softmax warps are at the next item
 // Rows of V behind a sequence's last key are zero in shared memory, so nothing stale is multiplied; rows of an item behind
-// its last one and keys behind the end have no say in the warps' votes: a sequence's bits do not depend on what lies beside it.
+// its last one and keys behind the end have no say in the warps' votes: the values that stand beside a sequence move no bit.
 //
 // Measured (32 query heads over 8 kv heads of 128, bf16): 2048 tokens over 65 000 keys 1.94 ms, 1106 TFLOP/s, 0.67 of the
 // measured bf16 rate (2.3 ms where the power cap holds the clock near 1.4 GHz); 12 packed documents of 50 to 4000 tokens
-// 577 us, 790 TFLOP/s. A unit takes about 3300 cycles, its four products 2048, a pipeline's softmax 1950.
+// 572 us, 798 TFLOP/s (626 us where calls follow without a pause). A unit takes about 3300 cycles, its four products 2048, a pipeline's softmax 1950.
 #include "attn_ragged.cuh"
 
 namespace b2 {
@@ -54,11 +55,6 @@ struct Cfg {
     static constexpr int OFF_BAR = (OFF_CUR + (int)sizeof(Cursor) + 15) / 16 * 16;
     static constexpr int SMEM = OFF_BAR + 256 + 1024;
 };
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-    const int n = ok ? 16 : 0;  // 0 source bytes: 16 zero bytes are written
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 
 template <int N>
 __device__ __forceinline__ uint64_t get2(const uint32_t (&v)[N], int e) {
@@ -972,7 +968,9 @@ int attn_tiles(RaggedArgs& a, int dim, bool bf16, void* workspace, cudaStream_t 
     const int mode = (a.softcap > 0.f ? 1 : 0) | (a.slopes ? 2 : 0) | (a.softcap > 128.f ? 4 : 0);
     ragged_slots(a, workspace, sm_count(), ROWS, dim);
     // A TMA box is as many rows as divide both a page and a unit; below 8 rows it would cut the swizzle's pattern, and a
-    // stride the map cannot hold has none: those caches are gathered by cp.async.
+    // stride the map cannot hold has none: those caches are gathered by cp.async (2048 tokens over 15 000 keys, 32 heads over 8
+    // of 128: pages of 64 by TMA 420 us, pages of 12 663, of 1 672). Queries of a group that does not divide 128 rows are gathered
+    // too, beside keys by TMA: 24 heads over 8, 335 us.
     a.box_rows = a.table ? a.page_size & -a.page_size : UNIT;
     if (a.box_rows > UNIT) a.box_rows = UNIT;
     CUtensorMap tq{}, tk{}, tv{};
