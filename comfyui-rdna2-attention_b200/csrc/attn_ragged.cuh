@@ -342,12 +342,16 @@ struct Pair;  // two 16-bit values of T from fp32, rounded to nearest even
 template <>
 struct Pair<__half> {
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return h2_as_u32(__floats2half2_rn(a, b)); }
+    static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(u32_as_h2(u)); }
 };
 template <>
 struct Pair<__nv_bfloat16> {
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t u) {
+        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
     }
 };
 

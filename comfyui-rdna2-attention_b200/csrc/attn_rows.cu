@@ -230,16 +230,26 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const 
                     x[t][e] = ex2_approx(x[t][e] - ref[e >> 1]);
                     l[e >> 1] += x[t][e];
                 }
-            // O += P V. P is rounded to the inputs' type for the product (its relative error, half a step of that
-            // type per key, averages over the row); the sum l keeps the fp32 values.
-            const uint32_t p[4] = {Pair<T>::pack(x[0][0], x[0][1]), Pair<T>::pack(x[0][2], x[0][3]),
-                                   Pair<T>::pack(x[1][0], x[1][1]), Pair<T>::pack(x[1][2], x[1][3])};
+            // O += P V, each weight as the sum of two values of the inputs' type (16 bits of it with bf16, 22 with fp16), so that
+            // the result is off by its own rounding only: 1.7e-3 of the values in the mean square with bf16, 2.3e-3 with weights
+            // of one part. The second product costs nothing beside the keys' loads at dim 128 (96 tokens over 500 to 16000 keys
+            // 449 us, 450 without it), 5 % at dim 64 (176.7, 168.5).
+            uint32_t p[4], r[4];
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                const float x0 = x[f >> 1][2 * (f & 1)], x1 = x[f >> 1][2 * (f & 1) + 1];
+                p[f] = Pair<T>::pack(x0, x1);
+                const float2 back = Pair<T>::unpack(p[f]);
+                r[f] = Pair<T>::pack(x0 - back.x, x1 - back.y);
+            }
 #pragma unroll
             for (int t = 0; t < D / 16; ++t) {
                 uint32_t b[4];
                 ldm4t(b, vt + chunk_at<D>((lane & 7) + (((lane >> 3) & 1) << 3), 2 * t + (lane >> 4)));
                 mma16816<T>(o[2 * t], p, b[0], b[1]);
                 mma16816<T>(o[2 * t + 1], p, b[2], b[3]);
+                mma16816<T>(o[2 * t], r, b[0], b[1]);
+                mma16816<T>(o[2 * t + 1], r, b[2], b[3]);
             }
         }
         cp_wait<0>();
