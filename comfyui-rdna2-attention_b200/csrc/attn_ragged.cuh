@@ -337,12 +337,21 @@ __device__ __forceinline__ uint64_t capped_pair(uint64_t y, float cap2) {
                fabsf(f.y) <= 1.f ? p.y : capped(f.y * (2.f * RAGGED_LOG2E), cap2));
 }
 
+// The fp32 value before x >= 0, and 0 for 0.
+__device__ __forceinline__ float below(float x) { return __uint_as_float(max(__float_as_uint(x), 1u) - 1u); }
+
 template <class T>
 struct Pair;  // two 16-bit values of T from fp32, rounded to nearest even
 template <>
 struct Pair<__half> {
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return h2_as_u32(__floats2half2_rn(a, b)); }
-    static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(u32_as_h2(u)); }
+    // a, b >= 0 as hi + lo, both positive where the weight is: hi is cut off below the value one fp32 step smaller. (A
+    // remainder of zero or less would turn an infinite value of a visible key into NaN.)
+    static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(below(b)), "f"(below(a)));
+        const float2 h = __half22float2(u32_as_h2(hi));
+        lo = pack(a - h.x, b - h.y);
+    }
 };
 template <>
 struct Pair<__nv_bfloat16> {
@@ -350,8 +359,10 @@ struct Pair<__nv_bfloat16> {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
-    static __device__ __forceinline__ float2 unpack(uint32_t u) {
-        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+        const uint32_t x = __float_as_uint(below(a)), y = __float_as_uint(below(b));
+        hi = __byte_perm(x, y, 0x7632);
+        lo = pack(a - __uint_as_float(x & 0xffff0000u), b - __uint_as_float(y & 0xffff0000u));
     }
 };
 

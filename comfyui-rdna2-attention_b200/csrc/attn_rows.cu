@@ -233,15 +233,10 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) attn_rows_kernel(const 
             // O += P V, each weight as the sum of two values of the inputs' type (16 bits of it with bf16, 22 with fp16), so that
             // the result is off by its own rounding only: 1.7e-3 of the values in the mean square with bf16, 2.3e-3 with weights
             // of one part. The second product costs nothing beside the keys' loads at dim 128 (96 tokens over 500 to 16000 keys
-            // 449 us, 450 without it), 5 % at dim 64 (176.7, 168.5).
+            // 461 us with and without it), 5 % at dim 64 (179, 169.5).
             uint32_t p[4], r[4];
 #pragma unroll
-            for (int f = 0; f < 4; ++f) {
-                const float x0 = x[f >> 1][2 * (f & 1)], x1 = x[f >> 1][2 * (f & 1) + 1];
-                p[f] = Pair<T>::pack(x0, x1);
-                const float2 back = Pair<T>::unpack(p[f]);
-                r[f] = Pair<T>::pack(x0 - back.x, x1 - back.y);
-            }
+            for (int f = 0; f < 4; ++f) Pair<T>::split(x[f >> 1][2 * (f & 1)], x[f >> 1][2 * (f & 1) + 1], p[f], r[f]);
 #pragma unroll
             for (int t = 0; t < D / 16; ++t) {
                 uint32_t b[4];

@@ -295,3 +295,21 @@ def test_few_rows_are_off_by_their_rounding(pkg, dev, dtype, D, keys):
     out = pkg.ops.attn_paged(q, kc, vc, table, cu, lengths)
     want = torch.cat([attend64(q[b:b + 1], pages_of(kc, table, b, keys), pages_of(vc, table, b, keys))[0] for b in range(B)])
     assert (out.double() - want).norm() < 1.02 * (want.to(dtype).double() - want).norm()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_infinite_values_of_visible_keys(pkg, dev, dtype, rows, D):
+    """An infinity in v comes out as itself where its key has weight (at least 2^-9 here), and touches its column only."""
+    m = 24
+    q, k, v = randn(dev, (1, 2, D), 97, dtype, 0.5), randn(dev, (m, 1, D), 98, dtype, 0.5), randn(dev, (m, 1, D), 99, dtype)
+    clean = v.clone()
+    v[3, 0, 5], v[7, 0, 9], v[0, 0, D - 1] = math.inf, -math.inf, math.inf
+    v[2, 0, 11] = torch.finfo(dtype).max
+    out = pkg.ops.attn_packed(q, k, v, starts(dev, 1), starts(dev, m), max_q=rows)
+    assert (out[0, :, 5] == math.inf).all() and (out[0, :, 9] == -math.inf).all() and (out[0, :, D - 1] == math.inf).all()
+    rest = [c for c in range(D) if c not in (5, 9, 11, D - 1)]
+    want, _, mass = attend64(q, k, clean)
+    attend_check(out[..., rest], want[..., rest], mass[..., rest], dtype, m, clean.abs().max().item())
+    assert torch.isfinite(out[..., 11]).all()
