@@ -1,9 +1,8 @@
 // Ragged attention for many rows per kv head (chunks of prompts, packed documents): 256 rows per item on tcgen05.
 //
 // With 256 rows an item does 1024 D flops per key against 4 D bytes of keys and values, 256 per byte: just where the tensor
-// cores become the bound (1654 TFLOP/s over 6.55 TB/s are 252), and well inside it as the other row tiles and query heads
-// find the same keys in L2. Two pipelines A and B work in ping-pong: while the softmax warps of one
-// work on its scores, the tensor core works for the other (S, P and O in TMEM, P written back over the consumed scores
+// cores become the bound (1654 TFLOP/s over 6.55 TB/s are 252), and well inside it as the other row tiles find the same
+// keys in L2. Two pipelines A and B work in ping-pong: while the softmax warps of one work on its scores, the tensor core works for the other (S, P and O in TMEM, P written back over the consumed scores
 // as the A operand of the second product). An item of more than 128 rows puts its first 128 on A and the others on B,
 // each over the units that its own rows see. An item of up to 128 rows (short chunks, drafts being checked), which HBM
 // bounds, puts its even units on A and the odd ones on B, and the two results are joined at the end.
@@ -19,7 +18,8 @@
 //
 // Measured (32 query heads over 8 kv heads of 128, bf16): 2048 tokens over 65 000 keys 1.94 ms, 1106 TFLOP/s, 0.67 of the
 // measured bf16 rate (2.3 ms where the power cap holds the clock near 1.4 GHz); 12 packed documents of 50 to 4000 tokens
-// 572 us, 798 TFLOP/s (626 us where calls follow without a pause). A unit takes about 3300 cycles, its four products 2048, a pipeline's softmax 1950.
+// 572 us, 798 TFLOP/s (626 us where calls follow without a pause). A unit of the long chunk takes about 3300 cycles, its four
+// products 2048, a pipeline's softmax 1950.
 #include "attn_ragged.cuh"
 
 namespace b2 {
