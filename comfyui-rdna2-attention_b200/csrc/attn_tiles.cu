@@ -2,10 +2,11 @@
 //
 // With 256 rows an item does 1024 D flops per key against 4 D bytes of keys and values, 256 per byte: just where the tensor
 // cores become the bound (1654 TFLOP/s over 6.55 TB/s are 252), and well inside it as the other row tiles find the same
-// keys in L2. Two pipelines A and B work in ping-pong: while the softmax warps of one work on its scores, the tensor core works for the other (S, P and O in TMEM, P written back over the consumed scores
-// as the A operand of the second product). An item of more than 128 rows puts its first 128 on A and the others on B,
-// each over the units that its own rows see. An item of up to 128 rows (short chunks, drafts being checked), which HBM
-// bounds, puts its even units on A and the odd ones on B, and the two results are joined at the end.
+// keys in L2. Two pipelines A and B work in ping-pong: while the softmax warps of one work on its scores, the tensor core
+// works for the other (S, P and O in TMEM, P written back over the consumed scores as the A operand of the second product).
+// An item of more than 128 rows puts its first 128 on A and the others on B, each over the units that its own rows see. An
+// item of up to 128 rows (short chunks, drafts being checked) puts its even units on A and the odd ones on B, and the two
+// results are joined at the end.
 //
 // One CTA per SM walks its run of units (attn_ragged.cuh); every barrier's phase counts on across the items.
 //   warps 0..3, 4..7  softmax of A and B: thread -> row, its 128 scores of a unit in registers
